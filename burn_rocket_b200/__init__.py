@@ -31,7 +31,7 @@ __all__ = [
     "pack_i8", "quantize_row_groups",
     "pack_qat", "matmul", "matmul_host", "attention", "attention_window",
     "attention_causal_window", "attention_window_block", "attention_causal_block",
-    "attention_raw", "q8_0_dequant", "quantize_rows_i8", "matmul_i8_acc", "check_device_errors",
+    "attention_raw", "attention_packed", "attention_paged", "kv_append", "q8_0_dequant", "quantize_rows_i8", "matmul_i8_acc", "check_device_errors",
     "mem_stats", "launch_count",
 ]
 
@@ -99,7 +99,13 @@ def _dev_ptr(t) -> int:
 # ----------------------------------------------------------------------------- init / pack
 def init(device: int = 0) -> None:
     """Create the engine on CUDA device `device` (burn_rocket::init, ext.rs:561-580)."""
+    global _device
     _check(_lib.load().rb_init(int(device)), "rb_init")
+    if _device is None:
+        _device = int(device)
+
+
+_device = None  # the engine's device, once init has run
 
 
 def _as_f32_host(w) -> np.ndarray:
@@ -347,6 +353,181 @@ def attention_causal_block(q, k, v, n_head, n_kv_heads, head_dim, scale, softcap
     """rocket_attention_causal_block (ext.rs:145-163)."""
     return attention_raw(q, k, v, n_head, n_kv_heads, head_dim, scale, softcap, MASK_CAUSAL_BLOCK, window,
                          q_start, kv_start, **kw)
+
+
+# ----------------------------------------------------------------------------- ragged batches, paged cache
+def _rows(op: str, what: str, t, width: int) -> None:
+    """A [tokens, width] CUDA tensor whose rows are contiguous (any row stride)."""
+    if t.dim() != 2 or t.shape[1] != width or (t.stride(1) != 1 and width > 1):
+        raise OpFailure(Error(op, _lib.RB_E_SHAPE), detail=f"{what} must be [tokens, {width}] with contiguous rows, "
+                        f"got {tuple(t.shape)}, strides {t.stride()}")
+
+
+def _ld(t) -> int:
+    """Row stride in elements (that of a single row says nothing)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _same(op: str, ref, tensors, dtype) -> None:
+    """Every tensor on ref's device and of the given dtype."""
+    dev = ref.device
+    if dev.type != "cuda":
+        raise OpFailure(Error(op, _lib.RB_E_SHAPE), detail="expected CUDA tensors")
+    if _device is not None and dev.index != _device:
+        raise OpFailure(Error(op, _lib.RB_E_SHAPE), detail=f"tensors on {dev}, the engine is on cuda:{_device}")
+    for what, t in tensors:
+        if t.device != dev or t.dtype != dtype:
+            raise OpFailure(Error(op, _lib.RB_E_SHAPE), detail=f"{what} must be {dtype} on {dev}, got {t.dtype} on {t.device}")
+
+
+def _lengths(op: str, q, cu, kv_len=None) -> int:
+    """Batch size of int32 sequence bounds [batch + 1] (and key counts [batch])."""
+    import torch
+    _same(op, q, [("cu", cu)] if kv_len is None else [("cu", cu), ("kv_len", kv_len)], torch.int32)
+    batch = cu.shape[0] - 1 if cu.dim() == 1 else -1
+    if batch < 0 or not cu.is_contiguous():
+        raise OpFailure(Error(op, _lib.RB_E_SHAPE), detail="cu must be a contiguous int32 [batch + 1]")
+    if kv_len is not None and (kv_len.shape != (batch,) or not kv_len.is_contiguous()):
+        raise OpFailure(Error(op, _lib.RB_E_SHAPE), detail=f"kv_len must be a contiguous int32 [{batch}]")
+    return batch
+
+
+def _cache(op: str, q, k_cache, v_cache, page_table, batch: int, n_kv_heads: int, head_dim: int):
+    """(page stride, pages, page size, table row stride) of a paged cache."""
+    import torch
+    _same(op, q, (("k_cache", k_cache), ("v_cache", v_cache)), q.dtype)
+    _same(op, q, (("page_table", page_table),), torch.int32)
+    shape, row = k_cache.shape, n_kv_heads * head_dim
+    want = (row, head_dim, 1)  # strides inside a page; a dimension of size 1 has none
+    if (len(shape) != 4 or shape[2] != n_kv_heads or shape[3] != head_dim or v_cache.shape != shape
+            or any(n > 1 and not a == b == w for n, a, b, w in zip(shape[1:], k_cache.stride()[1:],
+                                                                   v_cache.stride()[1:], want))
+            or (shape[0] > 1 and k_cache.stride(0) != v_cache.stride(0))):
+        raise OpFailure(Error(op, _lib.RB_E_SHAPE), detail="k_cache and v_cache must be alike, [pages, page_size, "
+                        f"{n_kv_heads}, {head_dim}] with contiguous pages, got {tuple(shape)} and {tuple(v_cache.shape)}")
+    if page_table.dim() != 2 or page_table.shape[0] != batch or not page_table.is_contiguous():
+        raise OpFailure(Error(op, _lib.RB_E_SHAPE), detail=f"page_table must be a contiguous int32 [{batch}, pages]")
+    return k_cache.stride(0) if shape[0] > 1 else shape[1] * row, shape[0], shape[1], page_table.shape[1]
+
+
+def kv_append(q, k, v, k_cache, v_cache, page_table, cu_q, kv_len, n_head: int, n_kv_heads: int, head_dim: int,
+              cos, sin, q_norm=None, k_norm=None, eps: float = 1e-6, q_out=None, stream=None):
+    """Append new tokens to a paged key/value cache, the per-head RMSNorm
+    (q_norm / k_norm, f32 [head_dim]; None = no norm) and the position rotation
+    applied on the way (rb_kv_append). Returns the rotated queries.
+
+    q [tokens, n_head*head_dim], k and v [tokens, n_kv_heads*head_dim] (f16 or
+    bf16, rows contiguous: slices of a fused projection will do) hold the new
+    tokens of all sequences back to back, sequence b's in rows cu_q[b] ..
+    cu_q[b+1] (int32 [batch+1]); kv_len[b] (int32) counts its keys with the new
+    tokens, which are the last ones. The caches are [pages, page_size,
+    n_kv_heads, head_dim], page_table int32 [batch, max_pages]; cos / sin f32
+    [positions, head_dim/2]. q_out=q rotates in place."""
+    import torch
+    op = "kv_append"
+    _same(op, q, (("k", k), ("v", v)), q.dtype)
+    batch = _lengths(op, q, cu_q, kv_len)
+    _rows(op, "q", q, n_head * head_dim)
+    _rows(op, "k", k, n_kv_heads * head_dim)
+    _rows(op, "v", v, n_kv_heads * head_dim)
+    tokens = q.shape[0]
+    if k.shape[0] != tokens or v.shape[0] != tokens:
+        raise OpFailure(Error(op, _lib.RB_E_SHAPE), tokens, detail="q, k and v must have the same number of tokens")
+    page_stride, pages, page_size, width = _cache(op, q, k_cache, v_cache, page_table, batch, n_kv_heads, head_dim)
+    norms = [(n, t) for n, t in (("q_norm", q_norm), ("k_norm", k_norm)) if t is not None]
+    _same(op, q, [("cos", cos), ("sin", sin)] + norms, torch.float32)
+    if cos.dim() != 2 or cos.shape[1] * 2 != head_dim or sin.shape != cos.shape or not (
+            cos.is_contiguous() and sin.is_contiguous()):
+        raise OpFailure(Error(op, _lib.RB_E_SHAPE), detail=f"cos and sin must be contiguous [positions, {head_dim // 2}]")
+    for what, t in norms:
+        if t.shape != (head_dim,) or not t.is_contiguous():
+            raise OpFailure(Error(op, _lib.RB_E_SHAPE), detail=f"{what} must be a contiguous [{head_dim}]")
+    if q_out is None:
+        q_out = torch.empty(tokens, n_head * head_dim, dtype=q.dtype, device=q.device)
+    else:
+        _same(op, q, (("q_out", q_out),), q.dtype)
+        _rows(op, "q_out", q_out, n_head * head_dim)
+        if q_out.shape[0] != tokens:
+            raise OpFailure(Error(op, _lib.RB_E_SHAPE), tokens, detail="q_out must have q's number of tokens")
+    rc = _lib.load().rb_kv_append(
+        q.data_ptr(), _ld(q), k.data_ptr(), _ld(k), v.data_ptr(), _ld(v), _dtype_code(q), tokens, batch,
+        cu_q.data_ptr(), kv_len.data_ptr(), n_head, n_kv_heads, head_dim,
+        None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), eps,
+        cos.data_ptr(), sin.data_ptr(), cos.shape[0], q_out.data_ptr(), _ld(q_out), k_cache.data_ptr(),
+        v_cache.data_ptr(), page_stride, pages, page_size, page_table.data_ptr(), width, _stream_on(q, stream))
+    _check(rc, op, tokens, head_dim, n_head)
+    return q_out
+
+
+def attention_paged(q, k_cache, v_cache, page_table, cu_q, kv_len, n_head: int, n_kv_heads: int, head_dim: int,
+                    scale: float, max_q: int, max_kv: int = 0, softcap: Optional[float] = None, window: int = -1,
+                    out=None, stream=None):
+    """Causal grouped-query attention of new tokens over a paged key/value cache
+    (rb_attention_paged): one token a sequence, chunks of prompts, or a mix.
+
+    q [tokens, n_head*head_dim] and the batch as kv_append takes them, after the
+    new tokens were appended. max_q bounds the new tokens of any sequence; max_kv
+    is the longest context expected (0: the table's width), which only guides how
+    the work is divided. window >= 0 lets a query see its last `window`
+    positions; a query that sees none is zero."""
+    import torch
+    op = "attention_paged"
+    _same(op, q, (), None)
+    batch = _lengths(op, q, cu_q, kv_len)
+    _rows(op, "q", q, n_head * head_dim)
+    page_stride, pages, page_size, width = _cache(op, q, k_cache, v_cache, page_table, batch, n_kv_heads, head_dim)
+    out = _out(op, q, out)
+    rc = _lib.load().rb_attention_paged(
+        q.data_ptr(), _ld(q), k_cache.data_ptr(), v_cache.data_ptr(), page_stride, pages, page_size,
+        page_table.data_ptr(), width, cu_q.data_ptr(), kv_len.data_ptr(), batch, q.shape[0], max_q, max_kv,
+        out.data_ptr(), _ld(out), _dtype_code(q), n_head, n_kv_heads, head_dim, scale, softcap or 0.0, window,
+        _stream_on(q, stream))
+    _check(rc, op, q.shape[0], max_kv, head_dim)
+    return out
+
+
+def attention_packed(q, k, v, cu_seqlens, n_head: int, n_kv_heads: int, head_dim: int, scale: float,
+                     softcap: Optional[float] = None, is_causal: bool = True, window: int = -1, out=None, stream=None):
+    """Grouped-query attention within each of several packed sequences (whole
+    prompts of different lengths, rb_attention_packed): rows cu_seqlens[b] ..
+    cu_seqlens[b+1] (int32 [batch+1]) of q [tokens, n_head*head_dim] and of k, v
+    [tokens, n_kv_heads*head_dim] belong to sequence b. window >= 0: the last
+    `window` keys (causal), or |t - j| <= window."""
+    import torch
+    op = "attention_packed"
+    _same(op, q, (("k", k), ("v", v)), q.dtype)
+    batch = _lengths(op, q, cu_seqlens)
+    _rows(op, "q", q, n_head * head_dim)
+    _rows(op, "k", k, n_kv_heads * head_dim)
+    _rows(op, "v", v, n_kv_heads * head_dim)
+    if k.shape[0] != q.shape[0] or v.shape[0] != q.shape[0]:
+        raise OpFailure(Error(op, _lib.RB_E_SHAPE), q.shape[0], detail="q, k and v must have the same number of tokens")
+    out = _out(op, q, out)
+    mode = MASK_CAUSAL_WINDOW if is_causal else MASK_WINDOW  # window < 0: no window
+    rc = _lib.load().rb_attention_packed(
+        q.data_ptr(), _ld(q), k.data_ptr(), _ld(k), v.data_ptr(), _ld(v), out.data_ptr(), _ld(out),
+        _dtype_code(q), batch, q.shape[0], cu_seqlens.data_ptr(), n_head, n_kv_heads, head_dim, scale, softcap or 0.0,
+        mode, window, _stream_on(q, stream))
+    _check(rc, op, q.shape[0], batch, head_dim)
+    return out
+
+
+def _out(op: str, q, out):
+    """The output buffer: q's shape and dtype, contiguous rows."""
+    import torch
+    if out is None:
+        return torch.empty(q.shape[0], q.shape[1], dtype=q.dtype, device=q.device)
+    _same(op, q, (("out", out),), q.dtype)
+    _rows(op, "out", out, q.shape[1])
+    if out.shape[0] != q.shape[0]:
+        raise OpFailure(Error(op, _lib.RB_E_SHAPE), q.shape[0], detail="out must have q's number of tokens")
+    return out
+
+
+def _stream_on(t, stream) -> int:
+    """The given stream, or the current one of t's device."""
+    import torch
+    return (stream if stream is not None else torch.cuda.current_stream(t.device)).cuda_stream
 
 
 # ----------------------------------------------------------------------------- codec surfaces

@@ -72,6 +72,12 @@ SIGNATURES = {
     "rb_pack_f32_q8_0_device": (_i64, [C.POINTER(_p), C.POINTER(_i64), _i, _i64]),
     "rb_attention_batched": (_i, [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _i, _i64, _i64, _i64, _i, _i, _i, _f, _f,
                                   _i, _i64, _i64, _i64, _p]),
+    "rb_kv_append": (_i, [_p, _i64, _p, _i64, _p, _i64, _i, _i64, _i64, _p, _p, _i, _i, _i, _p, _p, _f, _p, _p, _i64,
+                          _p, _i64, _p, _p, _i64, _i64, _i, _p, _i64, _p]),
+    "rb_attention_paged": (_i, [_p, _i64, _p, _p, _i64, _i64, _i, _p, _i64, _p, _p, _i64, _i64, _i64, _i64, _p, _i64,
+                                _i, _i, _i, _i, _f, _f, _i64, _p]),
+    "rb_attention_packed": (_i, [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _i, _i64, _i64, _p, _i, _i, _i, _f, _f, _i,
+                                 _i64, _p]),
     "rb_rms_norm": (_i, [_p, _i, _p, _f, _p, _i, _i64, _i64, _p]),
     "rb_pack_f32_w8a8_device": (_i64, [_p, _i64, _i64, _f, _f]),
     "rb_pack_i8": (_i64, [_p, _i64, _i64, _i64]),

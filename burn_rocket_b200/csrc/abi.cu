@@ -276,6 +276,17 @@ int w8a8_view(int64_t id, W8A8View* v) {
   return RB_OK;
 }
 
+int engine_view(EngineView* v) {
+  std::lock_guard<std::mutex> lk(g_mu);
+  Engine* e;
+  const int rc = ensure_engine(&e);
+  if (rc) return rc;
+  v->device = e->device;
+  v->num_sms = e->num_sms;
+  v->err = e->err;
+  return RB_OK;
+}
+
 static size_t dtype_bytes(int dt) {
   switch (dt) {
     case RB_DTYPE_F32: return 4;

@@ -155,6 +155,69 @@ struct AttnLaunch {
 // staged as 80 through [rows, heads, 72] maps, head_maps = 1).
 int launch_attention(const CUtensorMap* tm, const AttnLaunch& L, cudaStream_t stream);
 
+// Ragged batches (kv_append.cu, attention_ragged.cu, attention_decode.cu).
+// Band bounds at or past this value mean "no bound".
+constexpr int kRaggedNoBound = 1 << 30;
+
+struct RaggedBatch {
+  const int32_t* cu;      // [batch + 1] first token row of each sequence
+  const int32_t* kv_len;  // [batch] keys of each sequence, or null: its own tokens
+  int batch;
+  int tokens;             // rows of the token buffers
+  int max_q;              // most new tokens that a sequence may have
+  int max_kv;             // most keys that a sequence may have
+  uint32_t* err;
+};
+
+// Keys and values: token rows (table == null), or a paged cache of
+// [num_pages, page_size, n_kv_heads, head_dim] slots.
+struct KeyValues {
+  const uint16_t* k;
+  const uint16_t* v;
+  int64_t ldk, ldv;      // row strides in elements (paged: of a page's slots, equal)
+  const int32_t* table;  // [batch, ld_table] page ids
+  int64_t ld_table;
+  int64_t page_stride;   // elements
+  int page_shift;        // log2 of the page size
+  int num_pages;
+};
+
+struct AttnRagged {
+  RaggedBatch seqs;
+  KeyValues kv;
+  const uint16_t* q;
+  uint16_t* out;
+  int64_t ldq, ldo;
+  int n_head, n_kv_heads, head_dim;
+  int bf16;
+  float scale, softcap;
+  int dlo, dhi;          // visible iff dlo <= key - query <= dhi
+  int hint_kv;           // the longest sequence the caller expects: divides work, bounds nothing
+  int num_sms;
+};
+int launch_attention_ragged(const AttnRagged& a, cudaStream_t st);
+
+struct KvAppend {
+  RaggedBatch seqs;
+  const uint16_t* q;
+  const uint16_t* k;
+  const uint16_t* v;
+  int64_t ldq, ldk, ldv, ldo;
+  int n_head, n_kv_heads, head_dim;
+  int bf16;
+  const float* q_norm;   // null: no norm
+  const float* k_norm;
+  float eps;
+  const float* cos_t;    // [max_pos, head_dim / 2]
+  const float* sin_t;
+  int max_pos;
+  uint16_t* q_out;
+  uint16_t* k_cache;
+  uint16_t* v_cache;
+  KeyValues cache;       // geometry of the cache (its k, v pointers unused)
+};
+int launch_kv_append(const KvAppend& a, cudaStream_t st);
+
 // Glue (glue.cu).
 int launch_rms_norm(const void* x, int xdt, const float* w, float eps, void* y, int ydt, int64_t rows,
                     int d, cudaStream_t st);
@@ -203,6 +266,13 @@ struct W8A8View {
   int num_sms;
   int device;
 };
+struct EngineView {
+  int device;
+  int num_sms;
+  uint32_t* err;
+};
+// The engine of this process; makes its device current.
+int engine_view(EngineView* v);
 // Copies out what a W8A8 matmul needs of packed weight `id` (engine lock held
 // for the copy only; weights are never freed).
 int w8a8_view(int64_t id, W8A8View* v);

@@ -237,6 +237,72 @@ RB_API int rb_attention_batched(const void* q, int64_t ldq, const void* k, int64
  * the 8 columns past each head read as zeros) and the output keeps 72
  * columns. */
 
+/* ---- ragged batches and the paged key/value cache (no counterpart in the
+ * reference, whose ops take one sequence a call and keep no cache). Sequences
+ * of different lengths lie back to back: sequence b owns the token rows
+ * [cu[b], cu[b+1]), cu int32 [batch+1], non-decreasing; rows outside every
+ * sequence are left as they were, a sequence may be empty. All lengths and page
+ * ids are DEVICE data read by the kernels, so a captured graph replays with new
+ * ones. f16 and bf16 buffers; rows start on 16-byte boundaries (16-byte aligned
+ * base, row stride a multiple of 8 elements), so q, k and v may be column
+ * slices of one fused projection output. tokens == 0 or batch == 0 does nothing.
+ *
+ * The cache is two buffers of [num_pages, page_size, n_kv_heads, head_dim]
+ * slots, pages page_stride elements apart (page_size 16, 32, 64 or 128; head_dim
+ * 64 or 128); position j of sequence b lies in slot j % page_size of page
+ * page_table[b*ld_table + j/page_size]. Table entries past a sequence's last
+ * page are not read, slots past its last position may hold anything.
+ *
+ * What the device data says is checked on the device: a sequence with bounds
+ * outside the token rows, more keys than the table has slots, more than max_q
+ * tokens or (rb_kv_append) a position outside the angle table is skipped, a page
+ * id outside the cache is not followed (its keys and values read as zeros, its
+ * tokens are not stored), and rb_check_device_errors reports bad-shape.
+ *
+ * The calls allocate nothing and share no workspace: they may run at the same
+ * time on several streams and in several graphs. */
+
+/* Appends the new tokens of each sequence to the cache: token i of sequence b
+ * has position kv_len[b] - n_b + i (kv_len counts the new tokens, which are
+ * the last n_b of them). Its q heads go normed and rotated to q_out, its k heads
+ * likewise into the cache, its v heads unchanged. The norm is the per-head
+ * RMSNorm of rb_qk_norm_rope with weights f32 [head_dim], NULL = none; cos/sin
+ * are f32 [max_pos, head_dim/2] as for rb_rope. Arithmetic in f32, one rounding.
+ * q_out may be q itself (with ldq_out == ldq). Two tokens must not map to one
+ * slot. */
+RB_API int rb_kv_append(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
+                        int dtype, int64_t tokens, int64_t batch, const int32_t* cu_q, const int32_t* kv_len,
+                        int n_head, int n_kv_heads, int head_dim, const float* q_norm_w, const float* k_norm_w,
+                        float eps, const float* cos, const float* sin, int64_t max_pos, void* q_out,
+                        int64_t ldq_out, void* k_cache, void* v_cache, int64_t page_stride, int64_t num_pages,
+                        int page_size, const int32_t* page_table, int64_t ld_table, void* stream);
+
+/* Causal grouped-query attention of each sequence's new tokens (1 for a
+ * decode step, a chunk of a prompt, any mix) over its kv_len[b] cached
+ * positions, the new ones included: the query at position p sees the positions
+ * j <= p, with window >= 0 only p - window < j. A query that sees none
+ * (window 0, or n_b > kv_len[b]) is zero; unlike rb_attention there is no score
+ * clamp, and nothing that stands in a masked position reaches a row. softcap as
+ * rb_attention; scale must be positive. max_q bounds the new tokens of any
+ * sequence; max_kv is the longest kv_len expected (0: the table's width): it
+ * only guides how the work is divided. out must not be an input. */
+RB_API int rb_attention_paged(const void* q, int64_t ldq, const void* k_cache, const void* v_cache,
+                              int64_t page_stride, int64_t num_pages, int page_size, const int32_t* page_table,
+                              int64_t ld_table, const int32_t* cu_q, const int32_t* kv_len, int64_t batch,
+                              int64_t tokens, int64_t max_q, int64_t max_kv, void* out, int64_t ldo, int dtype,
+                              int n_head, int n_kv_heads, int head_dim, float scale, float softcap, int64_t window,
+                              void* stream);
+
+/* Grouped-query attention within each of `batch` packed sequences (whole
+ * prompts, images): q, k, v and out rows [cu_seqlens[b], cu_seqlens[b+1])
+ * belong to sequence b. mask_mode is RB_MASK_NONE, CAUSAL, WINDOW or
+ * CAUSAL_WINDOW (window < 0 = unwindowed), head_dim 64, 72 or 128; a query that
+ * sees no key is zero, otherwise as rb_attention_paged. */
+RB_API int rb_attention_packed(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
+                               void* out, int64_t ldo, int dtype, int64_t batch, int64_t tokens,
+                               const int32_t* cu_seqlens, int n_head, int n_kv_heads, int head_dim, float scale,
+                               float softcap, int mask_mode, int64_t window, void* stream);
+
 /* ---- glue ops of the RocketOps surface (ext.rs:70-83, 1054-1152; formulas
  * host.rs:15-72). Device buffers, any float dtype, asynchronous on `stream`. */
 

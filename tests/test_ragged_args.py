@@ -1,0 +1,95 @@
+"""What the ragged-batch entry points refuse, checked without a GPU: every
+argument check runs before the engine is asked for, and device addresses are
+never read on the host."""
+import pytest
+
+from burn_rocket_b200 import _lib
+
+P = 0x7000_0000_0000  # a 16-byte aligned address that nothing on the host reads
+
+
+def call(name, base, **change):
+    args = dict(base)
+    assert set(change) <= set(args), change
+    args.update(change)
+    return getattr(_lib.load(), name)(*args.values())
+
+
+APPEND = dict(q=P, ldq=2048, k=P + 64, ldk=1024, v=P + 128, ldv=1024, dtype=1, tokens=8, batch=2, cu=P, kv_len=P,
+              n_head=16, n_kv_heads=8, head_dim=128, q_norm=P, k_norm=None, eps=1e-6, cos=P, sin=P, max_pos=100,
+              q_out=P + 256, ldq_out=2048, k_cache=P, v_cache=P, page_stride=16 * 1024, num_pages=10, page_size=16,
+              table=P, ld_table=4, stream=None)
+PAGED = dict(q=P + 64, ldq=2048, k_cache=P, v_cache=P, page_stride=16 * 1024, num_pages=10, page_size=16, table=P,
+             ld_table=4, cu=P, kv_len=P, batch=2, tokens=8, max_q=4, max_kv=0, out=P + 256, ldo=2048, dtype=2,
+             n_head=16, n_kv_heads=8, head_dim=128, scale=0.1, softcap=0.0, window=-1, stream=None)
+PACKED = dict(q=P, ldq=4096, k=P + 64, ldk=4096, v=P + 128, ldv=4096, out=P + 256, ldo=2048, dtype=1, batch=2, tokens=8,
+              cu=P, n_head=16, n_kv_heads=8, head_dim=128, scale=0.1, softcap=0.0, mode=2, window=-1, stream=None)
+NAN, INF = float("nan"), float("inf")
+
+COMMON = [dict(dtype=0), dict(dtype=3), dict(tokens=-1), dict(batch=-1), dict(tokens=1 << 31), dict(n_head=15),
+          dict(n_head=0), dict(n_kv_heads=0), dict(n_head=-16), dict(n_head=2048, n_kv_heads=8), dict(cu=None)]
+CACHE = [dict(page_size=8), dict(page_size=48), dict(page_size=256), dict(page_size=0), dict(num_pages=0),
+         dict(ld_table=0), dict(table=None), dict(page_stride=16 * 1024 - 8), dict(page_stride=16 * 1024 + 4),
+         dict(k_cache=None), dict(v_cache=None), dict(k_cache=P + 8), dict(v_cache=P + 2), dict(head_dim=72),
+         dict(head_dim=96), dict(kv_len=None)]
+SOFTMAX = [dict(scale=0.0), dict(scale=-0.1), dict(scale=NAN), dict(scale=INF), dict(softcap=-1.0), dict(softcap=NAN),
+           dict(softcap=INF)]
+
+
+@pytest.mark.parametrize("change", COMMON + CACHE + [
+    dict(q=None), dict(k=None), dict(v=None), dict(q_out=None), dict(ldq=2040), dict(ldk=1020), dict(ldv=1028),
+    dict(q=P + 8), dict(k=P + 2), dict(q_out=P + 4), dict(cos=None), dict(sin=None), dict(cos=P + 4), dict(q_norm=P + 8),
+    dict(max_pos=0), dict(eps=NAN), dict(eps=-1.0), dict(q_out=P, ldq=4096)])
+def test_kv_append_refuses(change):
+    rc = call("rb_kv_append", APPEND, **change)
+    assert rc in (_lib.RB_E_SHAPE, _lib.RB_E_UNSUPPORTED), (rc, change)
+    assert _lib.last_error().startswith("kv_append:")
+
+
+@pytest.mark.parametrize("change", COMMON + CACHE + SOFTMAX + [
+    dict(q=None), dict(out=None), dict(ldq=1024), dict(ldo=2044), dict(q=P + 2), dict(out=P + 8), dict(out=P + 64),
+    dict(out=P), dict(max_q=-1), dict(max_kv=-1)])
+def test_attention_paged_refuses(change):
+    rc = call("rb_attention_paged", PAGED, **change)
+    assert rc in (_lib.RB_E_SHAPE, _lib.RB_E_UNSUPPORTED), (rc, change)
+    assert _lib.last_error().startswith("attention_paged:")
+
+
+@pytest.mark.parametrize("change", COMMON + SOFTMAX + [
+    dict(q=None), dict(k=None), dict(v=None), dict(out=None), dict(ldk=1000), dict(ldv=4092), dict(v=P + 4),
+    dict(out=P), dict(out=P + 64), dict(out=P + 128), dict(mode=1), dict(mode=5), dict(mode=6), dict(mode=7),
+    dict(mode=-1), dict(head_dim=80), dict(head_dim=0)])
+def test_attention_packed_refuses(change):
+    rc = call("rb_attention_packed", PACKED, **change)
+    assert rc in (_lib.RB_E_SHAPE, _lib.RB_E_UNSUPPORTED), (rc, change)
+    assert _lib.last_error().startswith("attention_packed:")
+
+
+@pytest.mark.parametrize("name,base", [("rb_kv_append", APPEND), ("rb_attention_paged", PAGED),
+                                       ("rb_attention_packed", PACKED)])
+def test_empty_batches_are_no_work(name, base):
+    assert call(name, base, tokens=0) == _lib.RB_OK
+    assert call(name, base, batch=0) == _lib.RB_OK
+
+
+def test_good_arguments_need_the_engine():
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("would launch on addresses that are not memory")
+    for name, base in (("rb_kv_append", APPEND), ("rb_attention_paged", PAGED), ("rb_attention_packed", PACKED)):
+        assert call(name, base) == _lib.RB_E_IO
+        assert "rb_init" in _lib.last_error()
+
+
+def test_python_refusals():
+    """The wrappers' own checks: shapes, dtypes, strides and devices."""
+    import torch
+    import burn_rocket_b200 as rb
+    q = torch.zeros(4, 256, dtype=torch.float16)
+    cu = torch.tensor([0, 4], dtype=torch.int32)
+    with pytest.raises(rb.OpFailure, match="CUDA"):
+        rb.attention_packed(q, q, q, cu, 2, 2, 128, 0.1)
+    with pytest.raises(rb.OpFailure, match="CUDA"):
+        rb.kv_append(q, q, q, q, q, cu, cu, cu, 2, 2, 128, q, q)
+    with pytest.raises(rb.OpFailure, match="CUDA"):
+        rb.attention_paged(q, q, q, cu, cu, cu, 2, 2, 128, 0.1, max_q=4)
