@@ -13,7 +13,7 @@ namespace ragged {
 
 // One warp per (token, head).
 template <int D, bool BF16, bool PAGED>
-__global__ void __launch_bounds__(256) rows_kernel(const AttnRagged p) {
+__global__ void __launch_bounds__(256) rows_kernel(const __grid_constant__ AttnRagged p) {
   const int64_t task = blockIdx.x * static_cast<int64_t>(blockDim.x >> 5) + (threadIdx.x >> 5);
   const int t = static_cast<int>(task / p.n_head), head = static_cast<int>(task % p.n_head);
   if (t >= p.seqs.tokens) return;
@@ -42,6 +42,8 @@ static int launch_rows(const AttnRagged& a, cudaStream_t st) {
 }  // namespace ragged
 
 int launch_attention_ragged(const AttnRagged& a, cudaStream_t st) {
+  if (a.kv.table && static_cast<int64_t>(a.seqs.max_q) * (a.n_head / a.n_kv_heads) <= 16)
+    return launch_attention_decode(a, st);
   if (a.head_dim == 128) return ragged::launch_rows<128>(a, st);
   if (a.head_dim == 64) return ragged::launch_rows<64>(a, st);
   if (a.head_dim == 72) return ragged::launch_rows<72>(a, st);

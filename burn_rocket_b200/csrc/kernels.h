@@ -196,6 +196,7 @@ struct AttnRagged {
   int num_sms;
 };
 int launch_attention_ragged(const AttnRagged& a, cudaStream_t st);
+int launch_attention_decode(const AttnRagged& a, cudaStream_t st);  // paged, few rows a sequence
 
 struct KvAppend {
   RaggedBatch seqs;

@@ -89,9 +89,11 @@ __device__ __forceinline__ uint16_t f2h(float x) {
 // One query row by one warp, from the definition: scores, softmax statistics
 // and sums in f32, one rounding at the end. Only the visible keys and values
 // are read, so nothing that stands in a masked place can reach the row; a row
-// that sees no key is zero. Lane l holds the columns l, l + 32, ...
+// that sees no key is zero. Lane l holds the columns l, l + 32, ...; the columns
+// [c0, c1) are written.
 template <int D, bool BF16, bool PAGED>
-__device__ void row_attention(const AttnRagged& p, int b, const Seq& s, int i, int head) {
+__device__ __noinline__ void row_attention(const AttnRagged& p, int b, const Seq& s, int i, int head, int c0 = 0,
+                                           int c1 = D) {
   constexpr int NC = (D + 31) / 32;
   const int lane = threadIdx.x & 31;
   const int g = head / (p.n_head / p.n_kv_heads);
@@ -150,7 +152,7 @@ __device__ void row_attention(const AttnRagged& p, int b, const Seq& s, int i, i
   const float inv = lo > hi ? 0.0f : 1.0f / l;
 #pragma unroll
   for (int c = 0; c < NC; ++c)
-    if (lane + 32 * c < D) out[lane + 32 * c] = f2h<BF16>(lo > hi ? 0.0f : acc[c] * inv);
+    if (lane + 32 * c >= c0 && lane + 32 * c < c1) out[lane + 32 * c] = f2h<BF16>(lo > hi ? 0.0f : acc[c] * inv);
 }
 
 }  // namespace rb
