@@ -112,6 +112,25 @@ int make_tmap_heads(CUtensorMap* map, const void* base, uint64_t rows, uint64_t 
   return RB_OK;
 }
 
+int make_tmap_16bit(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const uint64_t* strides_bytes,
+                    const uint32_t* box, int swizzle_bytes) {
+  if (!load_encode_fn()) return fail(RB_E_DEVICE, "cuTensorMapEncodeTiled unavailable");
+  cuuint64_t d[5], s[5];
+  cuuint32_t b[5];
+  const cuuint32_t one[5] = {1, 1, 1, 1, 1};
+  for (int i = 0; i < rank; ++i) {
+    d[i] = dims[i];
+    b[i] = box[i];
+    if (i) s[i - 1] = strides_bytes[i - 1];
+  }
+  const CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, rank, const_cast<void*>(base), d, s, b, one,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              swizzle_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_32B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(RB_E_DEVICE, "cuTensorMapEncodeTiled failed (%d), %d dimensions", (int)r, rank);
+  return RB_OK;
+}
+
 int bn_index(int bn) {
   switch (bn) {
     case 256: return 0;

@@ -1,53 +1,66 @@
-// attention_ragged.cu — attention over a ragged batch: packed whole prompts,
-// or new tokens over a paged key/value cache.
-//
-//   out_i = sum_j softmax_j(cap(scale q_i . k_j)) v_j
-//
-// over the keys j that the mask lets query i see (one interval per query); a
-// query that sees none is zero.
-#include "ragged.cuh"
+// attention_ragged.cu — which kernel a ragged-batch attention call runs, its
+// tensor maps and how its work is divided.
+#include "attention_tile.cuh"
 
 namespace rb {
 
-namespace ragged {
-
-// One warp per (token, head).
-template <int D, bool BF16, bool PAGED>
-__global__ void __launch_bounds__(256) rows_kernel(const __grid_constant__ AttnRagged p) {
-  const int64_t task = blockIdx.x * static_cast<int64_t>(blockDim.x >> 5) + (threadIdx.x >> 5);
-  const int t = static_cast<int>(task / p.n_head), head = static_cast<int>(task % p.n_head);
-  if (t >= p.seqs.tokens) return;
-  const int b = find_seq(p.seqs.cu, p.seqs.batch, t);
-  if (b < 0) return;
-  const Seq s = load_seq(p.seqs, b);
-  if (t - s.q0 < s.n) row_attention<D, BF16, PAGED>(p, b, s, t - s.q0, head);
-}
-
-template <int D>
-static int launch_rows(const AttnRagged& a, cudaStream_t st) {
-  const int64_t blocks = (static_cast<int64_t>(a.seqs.tokens) * a.n_head + 7) / 8;
-  if (blocks > 0x7fffffff) return RB_E_SHAPE;
-  const dim3 grid(static_cast<unsigned>(blocks));
-  if (a.kv.table) {
-    if (a.bf16) rows_kernel<D, true, true><<<grid, 256, 0, st>>>(a);
-    else rows_kernel<D, false, true><<<grid, 256, 0, st>>>(a);
+static int launch_attention_tile(const AttnRagged& a, cudaStream_t st) {
+  using namespace tile;
+  TileParams p{};
+  p.a = a;
+  p.group = a.n_head / a.n_kv_heads;
+  p.tq = BM / p.group;
+  const int d = a.head_dim, span = 2 * p.tq;
+  const uint64_t tokens = a.seqs.tokens, row = 2ull * d;
+  CUtensorMap tm[6];
+  auto maps = [&](int at, uint32_t cols, int swizzle) -> int {
+    int rc;
+    {
+      const uint64_t dims[3] = {uint64_t(d), uint64_t(a.n_head), tokens}, strides[2] = {row, 2ull * a.ldq};
+      const uint32_t box[3] = {cols, uint32_t(p.group), uint32_t(p.tq)};
+      if ((rc = make_tmap_16bit(&tm[at], a.q, 3, dims, strides, box, swizzle)) != RB_OK) return rc;
+    }
+    for (int i = 0; i < 2; ++i) {
+      const void* base = i ? a.kv.v : a.kv.k;
+      const uint64_t ld = 2ull * (i ? a.kv.ldv : a.kv.ldk);
+      if (a.kv.table) {
+        const uint32_t page = 1u << a.kv.page_shift;
+        const uint64_t dims[4] = {uint64_t(d), uint64_t(a.n_kv_heads), page, uint64_t(a.kv.num_pages)};
+        const uint64_t strides[3] = {row, ld, 2ull * a.kv.page_stride};
+        const uint32_t box[4] = {cols, 1, page, 1};
+        rc = make_tmap_16bit(&tm[at + 1 + i], base, 4, dims, strides, box, swizzle);
+      } else {
+        const uint64_t dims[3] = {uint64_t(d), uint64_t(a.n_kv_heads), tokens}, strides[2] = {row, ld};
+        const uint32_t box[3] = {cols, 1, uint32_t(BN)};
+        rc = make_tmap_16bit(&tm[at + 1 + i], base, 3, dims, strides, box, swizzle);
+      }
+      if (rc != RB_OK) return rc;
+    }
+    return RB_OK;
+  };
+  int rc = maps(0, 64, 128);
+  if (rc != RB_OK) return rc;
+  if (d == 72) {
+    if ((rc = maps(3, 16, 32)) != RB_OK) return rc;
   } else {
-    if (a.bf16) rows_kernel<D, true, false><<<grid, 256, 0, st>>>(a);
-    else rows_kernel<D, false, false><<<grid, 256, 0, st>>>(a);
+    for (int i = 0; i < 3; ++i) tm[3 + i] = tm[i];
   }
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? RB_OK : report_error(RB_E_DEVICE, cudaGetErrorString(e));
+  // At most this many units: every sequence ends in one part-filled span.
+  const int64_t units = (static_cast<int64_t>(a.seqs.tokens) / span + std::min(a.seqs.batch, a.seqs.tokens)) * a.n_kv_heads;
+  if (units > 0x7fffffff) return report_error(RB_E_SHAPE, "ragged attention: batch too large");
+  // Fewer units than half the SMs: a cluster a unit, two key tiles a CTA at least.
+  int ranks = 1;
+  const int keys = a.dlo <= -kRaggedNoBound ? a.hint_kv : std::min(a.hint_kv, span - 1 - a.dlo + std::max(a.dhi, 0));
+  while (ranks < 8 && units * ranks * 2 <= a.num_sms && keys >= ranks * 4 * BN) ranks *= 2;
+  const unsigned grid = static_cast<unsigned>(ranks > 1 ? units * ranks : std::min<int64_t>(units, a.num_sms));
+  if (d == 128) return launch_d128(tm, p, grid, ranks, st);
+  return d == 64 ? launch_d64(tm, p, grid, ranks, st) : launch_d80(tm, p, grid, ranks, st);
 }
-
-}  // namespace ragged
 
 int launch_attention_ragged(const AttnRagged& a, cudaStream_t st) {
   if (a.kv.table && static_cast<int64_t>(a.seqs.max_q) * (a.n_head / a.n_kv_heads) <= 16)
     return launch_attention_decode(a, st);
-  if (a.head_dim == 128) return ragged::launch_rows<128>(a, st);
-  if (a.head_dim == 64) return ragged::launch_rows<64>(a, st);
-  if (a.head_dim == 72) return ragged::launch_rows<72>(a, st);
-  return RB_E_UNSUPPORTED;
+  return launch_attention_tile(a, st);
 }
 
 }  // namespace rb

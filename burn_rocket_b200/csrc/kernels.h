@@ -155,7 +155,7 @@ struct AttnLaunch {
 // staged as 80 through [rows, heads, 72] maps, head_maps = 1).
 int launch_attention(const CUtensorMap* tm, const AttnLaunch& L, cudaStream_t stream);
 
-// Ragged batches (kv_append.cu, attention_ragged.cu, attention_decode.cu).
+// Ragged batches (kv_append.cu, attention_ragged.cu, attention_tile.cuh, attention_decode.cu).
 // Band bounds at or past this value mean "no bound".
 constexpr int kRaggedNoBound = 1 << 30;
 
@@ -249,6 +249,10 @@ int launch_last_token_l2(const float* x, int d, int seq, int batch, const float*
 int make_tmap_2d(CUtensorMap* map, const void* base, int elem_bytes, uint64_t rows,
                  uint64_t cols, uint64_t row_stride_elems, uint32_t box_cols, uint32_t box_rows,
                  int swizzle_bytes);  // 0 (none), 32, 64 or 128
+// Tiled map of 16-bit elements of any rank (dims and box innermost first,
+// strides in bytes from the second dimension on); swizzle 128 or 32 bytes.
+int make_tmap_16bit(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const uint64_t* strides_bytes,
+                    const uint32_t* box, int swizzle_bytes);
 // Index of an N tile in the per-weight tensor-map caches ({256,128,96,64}).
 int bn_index(int bn);
 
