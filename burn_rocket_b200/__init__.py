@@ -356,58 +356,73 @@ def attention_causal_block(q, k, v, n_head, n_kv_heads, head_dim, scale, softcap
 
 
 # ----------------------------------------------------------------------------- ragged batches, paged cache
-def _rows(op: str, what: str, t, width: int) -> None:
-    """A [tokens, width] CUDA tensor whose rows are contiguous (any row stride)."""
-    if t.dim() != 2 or t.shape[1] != width or (t.stride(1) != 1 and width > 1):
-        raise OpFailure(Error(op, _lib.RB_E_SHAPE), detail=f"{what} must be [tokens, {width}] with contiguous rows, "
-                        f"got {tuple(t.shape)}, strides {t.stride()}")
+def _refuse(op: str, detail: str, m: int = 0):
+    raise OpFailure(Error(op, _lib.RB_E_SHAPE), m, detail=detail)
 
 
-def _ld(t) -> int:
-    """Row stride in elements (that of a single row says nothing)."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _on(op: str, dev: int, dtype, **tensors) -> None:
+    """Every tensor on CUDA device `dev` and of the given dtype."""
+    for what, t in tensors.items():
+        if t.dtype is not dtype or t.get_device() != dev or not t.is_cuda:
+            _refuse(op, f"{what} must be {dtype} on cuda:{dev}, got {t.dtype} on {t.device}")
 
 
-def _same(op: str, ref, tensors, dtype) -> None:
-    """Every tensor on ref's device and of the given dtype."""
-    dev = ref.device
-    if dev.type != "cuda":
-        raise OpFailure(Error(op, _lib.RB_E_SHAPE), detail="expected CUDA tensors")
-    if _device is not None and dev.index != _device:
-        raise OpFailure(Error(op, _lib.RB_E_SHAPE), detail=f"tensors on {dev}, the engine is on cuda:{_device}")
-    for what, t in tensors:
-        if t.device != dev or t.dtype != dtype:
-            raise OpFailure(Error(op, _lib.RB_E_SHAPE), detail=f"{what} must be {dtype} on {dev}, got {t.dtype} on {t.device}")
+def _rows(op: str, what: str, t, tokens: int, width: int) -> int:
+    """Row stride in elements of [tokens, width] rows, each contiguous."""
+    if t.shape != (tokens, width):
+        _refuse(op, f"{what} must be [{tokens}, {width}], got {tuple(t.shape)}", tokens)
+    ld, step = t.stride()
+    if step != 1 and width > 1:
+        _refuse(op, f"{what} must have contiguous rows, got strides {(ld, step)}", tokens)
+    return ld if tokens > 1 else width  # (the stride of a single row says nothing)
 
 
-def _lengths(op: str, q, cu, kv_len=None) -> int:
-    """Batch size of int32 sequence bounds [batch + 1] (and key counts [batch])."""
+def _device_of(op: str, q) -> int:
+    if not q.is_cuda or q.dim() != 2:
+        _refuse(op, "expected 2-D CUDA tensors")
+    dev = q.get_device()
+    if _device is not None and dev != _device:
+        _refuse(op, f"tensors on cuda:{dev}, the engine is on cuda:{_device}")
+    return dev
+
+
+def _bounds(op: str, dev: int, cu) -> int:
+    """Batch size of sequence bounds int32 [batch + 1]."""
     import torch
-    _same(op, q, [("cu", cu)] if kv_len is None else [("cu", cu), ("kv_len", kv_len)], torch.int32)
-    batch = cu.shape[0] - 1 if cu.dim() == 1 else -1
-    if batch < 0 or not cu.is_contiguous():
-        raise OpFailure(Error(op, _lib.RB_E_SHAPE), detail="cu must be a contiguous int32 [batch + 1]")
-    if kv_len is not None and (kv_len.shape != (batch,) or not kv_len.is_contiguous()):
-        raise OpFailure(Error(op, _lib.RB_E_SHAPE), detail=f"kv_len must be a contiguous int32 [{batch}]")
-    return batch
+    _on(op, dev, torch.int32, cu=cu)
+    if cu.dim() != 1 or cu.shape[0] < 1 or not cu.is_contiguous():
+        _refuse(op, f"cu must be a contiguous int32 [batch + 1], got {tuple(cu.shape)}")
+    return cu.shape[0] - 1
 
 
-def _cache(op: str, q, k_cache, v_cache, page_table, batch: int, n_kv_heads: int, head_dim: int):
-    """(page stride, pages, page size, table row stride) of a paged cache."""
+def _cache(op: str, dev: int, dtype, k_cache, v_cache, page_table, kv_len, batch: int, n_kv_heads: int, head_dim: int):
+    """(page stride, pages, page size, table width) of a paged cache."""
     import torch
-    _same(op, q, (("k_cache", k_cache), ("v_cache", v_cache)), q.dtype)
-    _same(op, q, (("page_table", page_table),), torch.int32)
-    shape, row = k_cache.shape, n_kv_heads * head_dim
-    want = (row, head_dim, 1)  # strides inside a page; a dimension of size 1 has none
-    if (len(shape) != 4 or shape[2] != n_kv_heads or shape[3] != head_dim or v_cache.shape != shape
-            or any(n > 1 and not a == b == w for n, a, b, w in zip(shape[1:], k_cache.stride()[1:],
-                                                                   v_cache.stride()[1:], want))
-            or (shape[0] > 1 and k_cache.stride(0) != v_cache.stride(0))):
-        raise OpFailure(Error(op, _lib.RB_E_SHAPE), detail="k_cache and v_cache must be alike, [pages, page_size, "
-                        f"{n_kv_heads}, {head_dim}] with contiguous pages, got {tuple(shape)} and {tuple(v_cache.shape)}")
+    _on(op, dev, dtype, k_cache=k_cache, v_cache=v_cache)
+    _on(op, dev, torch.int32, page_table=page_table, kv_len=kv_len)
+    shape, strides = k_cache.shape, k_cache.stride()
+    row = n_kv_heads * head_dim
+    ok = len(shape) == 4 and shape[2] == n_kv_heads and shape[3] == head_dim and v_cache.shape == shape
+    if ok and not (strides[1:] == (row, head_dim, 1) and v_cache.stride() == strides):
+        # A dimension of size 1 has no stride to speak of.
+        ok = all(n <= 1 or (a == b and (i == 0 or a == (row, head_dim, 1)[i - 1]))
+                 for i, (n, a, b) in enumerate(zip(shape, strides, v_cache.stride())))
+    if not ok:
+        _refuse(op, f"k_cache and v_cache must be alike, [pages, page_size, {n_kv_heads}, {head_dim}] with contiguous "
+                f"pages, got {tuple(shape)} and {tuple(v_cache.shape)}")
     if page_table.dim() != 2 or page_table.shape[0] != batch or not page_table.is_contiguous():
-        raise OpFailure(Error(op, _lib.RB_E_SHAPE), detail=f"page_table must be a contiguous int32 [{batch}, pages]")
-    return k_cache.stride(0) if shape[0] > 1 else shape[1] * row, shape[0], shape[1], page_table.shape[1]
+        _refuse(op, f"page_table must be a contiguous int32 [{batch}, pages], got {tuple(page_table.shape)}")
+    if kv_len.shape != (batch,) or not kv_len.is_contiguous():
+        _refuse(op, f"kv_len must be a contiguous int32 [{batch}], got {tuple(kv_len.shape)}")
+    return strides[0] if shape[0] > 1 else shape[1] * row, shape[0], shape[1], page_table.shape[1]
+
+
+def _stream_on(dev: int, stream) -> int:
+    """The given stream, or the current one of device `dev`."""
+    if stream is not None:
+        return stream.cuda_stream
+    import torch
+    return torch.cuda.current_stream(dev).cuda_stream
 
 
 def kv_append(q, k, v, k_cache, v_cache, page_table, cu_q, kv_len, n_head: int, n_kv_heads: int, head_dim: int,
@@ -425,37 +440,33 @@ def kv_append(q, k, v, k_cache, v_cache, page_table, cu_q, kv_len, n_head: int, 
     [positions, head_dim/2]. q_out=q rotates in place."""
     import torch
     op = "kv_append"
-    _same(op, q, (("k", k), ("v", v)), q.dtype)
-    batch = _lengths(op, q, cu_q, kv_len)
-    _rows(op, "q", q, n_head * head_dim)
-    _rows(op, "k", k, n_kv_heads * head_dim)
-    _rows(op, "v", v, n_kv_heads * head_dim)
-    tokens = q.shape[0]
-    if k.shape[0] != tokens or v.shape[0] != tokens:
-        raise OpFailure(Error(op, _lib.RB_E_SHAPE), tokens, detail="q, k and v must have the same number of tokens")
-    page_stride, pages, page_size, width = _cache(op, q, k_cache, v_cache, page_table, batch, n_kv_heads, head_dim)
-    norms = [(n, t) for n, t in (("q_norm", q_norm), ("k_norm", k_norm)) if t is not None]
-    _same(op, q, [("cos", cos), ("sin", sin)] + norms, torch.float32)
-    if cos.dim() != 2 or cos.shape[1] * 2 != head_dim or sin.shape != cos.shape or not (
-            cos.is_contiguous() and sin.is_contiguous()):
-        raise OpFailure(Error(op, _lib.RB_E_SHAPE), detail=f"cos and sin must be contiguous [positions, {head_dim // 2}]")
-    for what, t in norms:
-        if t.shape != (head_dim,) or not t.is_contiguous():
-            raise OpFailure(Error(op, _lib.RB_E_SHAPE), detail=f"{what} must be a contiguous [{head_dim}]")
+    dev, dtype, tokens = _device_of(op, q), q.dtype, q.shape[0]
+    batch = _bounds(op, dev, cu_q)
+    page_stride, pages, page_size, width = _cache(op, dev, dtype, k_cache, v_cache, page_table, kv_len, batch,
+                                                  n_kv_heads, head_dim)
     if q_out is None:
-        q_out = torch.empty(tokens, n_head * head_dim, dtype=q.dtype, device=q.device)
-    else:
-        _same(op, q, (("q_out", q_out),), q.dtype)
-        _rows(op, "q_out", q_out, n_head * head_dim)
-        if q_out.shape[0] != tokens:
-            raise OpFailure(Error(op, _lib.RB_E_SHAPE), tokens, detail="q_out must have q's number of tokens")
-    rc = _lib.load().rb_kv_append(
-        q.data_ptr(), _ld(q), k.data_ptr(), _ld(k), v.data_ptr(), _ld(v), _dtype_code(q), tokens, batch,
-        cu_q.data_ptr(), kv_len.data_ptr(), n_head, n_kv_heads, head_dim,
-        None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), eps,
-        cos.data_ptr(), sin.data_ptr(), cos.shape[0], q_out.data_ptr(), _ld(q_out), k_cache.data_ptr(),
-        v_cache.data_ptr(), page_stride, pages, page_size, page_table.data_ptr(), width, _stream_on(q, stream))
-    _check(rc, op, tokens, head_dim, n_head)
+        q_out = torch.empty(tokens, n_head * head_dim, dtype=dtype, device=q.device)
+    _on(op, dev, dtype, k=k, v=v, q_out=q_out)
+    _on(op, dev, torch.float32, cos=cos, sin=sin)
+    if cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] * 2 != head_dim or not (
+            cos.is_contiguous() and sin.is_contiguous()):
+        _refuse(op, f"cos and sin must be contiguous [positions, {head_dim // 2}]")
+    norms = [0, 0]
+    for i, t in enumerate((q_norm, k_norm)):
+        if t is not None:
+            _on(op, dev, torch.float32, norm=t)
+            if t.shape != (head_dim,) or not t.is_contiguous():
+                _refuse(op, f"norm weights must be contiguous [{head_dim}], got {tuple(t.shape)}")
+            norms[i] = t.data_ptr()
+    args = _lib.KV_APPEND_ARGS.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), _rows(op, "q", q, tokens, n_head * head_dim),
+        _rows(op, "k", k, tokens, n_kv_heads * head_dim), _rows(op, "v", v, tokens, n_kv_heads * head_dim), tokens, batch,
+        cu_q.data_ptr(), kv_len.data_ptr(), norms[0], norms[1], cos.data_ptr(), sin.data_ptr(), cos.shape[0],
+        q_out.data_ptr(), _rows(op, "q_out", q_out, tokens, n_head * head_dim), k_cache.data_ptr(), v_cache.data_ptr(),
+        page_stride, pages, page_table.data_ptr(), width, _dtype_code(q), n_head, n_kv_heads, head_dim, page_size, eps)
+    rc = _lib.load().rb_kv_append(args, _stream_on(dev, stream))
+    if rc:
+        _check(rc, op, tokens, head_dim, n_head)
     return q_out
 
 
@@ -470,19 +481,20 @@ def attention_paged(q, k_cache, v_cache, page_table, cu_q, kv_len, n_head: int, 
     is the longest context expected (0: the table's width), which only guides how
     the work is divided. window >= 0 lets a query see its last `window`
     positions; a query that sees none is zero."""
-    import torch
     op = "attention_paged"
-    _same(op, q, (), None)
-    batch = _lengths(op, q, cu_q, kv_len)
-    _rows(op, "q", q, n_head * head_dim)
-    page_stride, pages, page_size, width = _cache(op, q, k_cache, v_cache, page_table, batch, n_kv_heads, head_dim)
-    out = _out(op, q, out)
-    rc = _lib.load().rb_attention_paged(
-        q.data_ptr(), _ld(q), k_cache.data_ptr(), v_cache.data_ptr(), page_stride, pages, page_size,
-        page_table.data_ptr(), width, cu_q.data_ptr(), kv_len.data_ptr(), batch, q.shape[0], max_q, max_kv,
-        out.data_ptr(), _ld(out), _dtype_code(q), n_head, n_kv_heads, head_dim, scale, softcap or 0.0, window,
-        _stream_on(q, stream))
-    _check(rc, op, q.shape[0], max_kv, head_dim)
+    dev, dtype, tokens = _device_of(op, q), q.dtype, q.shape[0]
+    batch = _bounds(op, dev, cu_q)
+    page_stride, pages, page_size, width = _cache(op, dev, dtype, k_cache, v_cache, page_table, kv_len, batch,
+                                                  n_kv_heads, head_dim)
+    out = _out(op, dev, q, out)
+    args = _lib.ATTENTION_PAGED_ARGS.pack(
+        q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+        _rows(op, "q", q, tokens, n_head * head_dim), _rows(op, "out", out, tokens, n_head * head_dim), tokens, batch,
+        cu_q.data_ptr(), kv_len.data_ptr(), max_q, max_kv, page_stride, pages, page_table.data_ptr(), width, window,
+        _dtype_code(q), n_head, n_kv_heads, head_dim, page_size, scale, softcap or 0.0)
+    rc = _lib.load().rb_attention_paged(args, _stream_on(dev, stream))
+    if rc:
+        _check(rc, op, tokens, max_kv, head_dim)
     return out
 
 
@@ -493,41 +505,29 @@ def attention_packed(q, k, v, cu_seqlens, n_head: int, n_kv_heads: int, head_dim
     cu_seqlens[b+1] (int32 [batch+1]) of q [tokens, n_head*head_dim] and of k, v
     [tokens, n_kv_heads*head_dim] belong to sequence b. window >= 0: the last
     `window` keys (causal), or |t - j| <= window."""
-    import torch
     op = "attention_packed"
-    _same(op, q, (("k", k), ("v", v)), q.dtype)
-    batch = _lengths(op, q, cu_seqlens)
-    _rows(op, "q", q, n_head * head_dim)
-    _rows(op, "k", k, n_kv_heads * head_dim)
-    _rows(op, "v", v, n_kv_heads * head_dim)
-    if k.shape[0] != q.shape[0] or v.shape[0] != q.shape[0]:
-        raise OpFailure(Error(op, _lib.RB_E_SHAPE), q.shape[0], detail="q, k and v must have the same number of tokens")
-    out = _out(op, q, out)
-    mode = MASK_CAUSAL_WINDOW if is_causal else MASK_WINDOW  # window < 0: no window
-    rc = _lib.load().rb_attention_packed(
-        q.data_ptr(), _ld(q), k.data_ptr(), _ld(k), v.data_ptr(), _ld(v), out.data_ptr(), _ld(out),
-        _dtype_code(q), batch, q.shape[0], cu_seqlens.data_ptr(), n_head, n_kv_heads, head_dim, scale, softcap or 0.0,
-        mode, window, _stream_on(q, stream))
-    _check(rc, op, q.shape[0], batch, head_dim)
+    dev, dtype, tokens = _device_of(op, q), q.dtype, q.shape[0]
+    batch = _bounds(op, dev, cu_seqlens)
+    out = _out(op, dev, q, out)
+    _on(op, dev, dtype, k=k, v=v)
+    args = _lib.ATTENTION_PACKED_ARGS.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _rows(op, "q", q, tokens, n_head * head_dim),
+        _rows(op, "k", k, tokens, n_kv_heads * head_dim), _rows(op, "v", v, tokens, n_kv_heads * head_dim),
+        _rows(op, "out", out, tokens, n_head * head_dim), tokens, batch, cu_seqlens.data_ptr(), window, _dtype_code(q),
+        n_head, n_kv_heads, head_dim, MASK_CAUSAL_WINDOW if is_causal else MASK_WINDOW, scale, softcap or 0.0)
+    rc = _lib.load().rb_attention_packed(args, _stream_on(dev, stream))
+    if rc:
+        _check(rc, op, tokens, batch, head_dim)
     return out
 
 
-def _out(op: str, q, out):
-    """The output buffer: q's shape and dtype, contiguous rows."""
-    import torch
+def _out(op: str, dev: int, q, out):
+    """The output buffer: q's shape and dtype."""
     if out is None:
-        return torch.empty(q.shape[0], q.shape[1], dtype=q.dtype, device=q.device)
-    _same(op, q, (("out", out),), q.dtype)
-    _rows(op, "out", out, q.shape[1])
-    if out.shape[0] != q.shape[0]:
-        raise OpFailure(Error(op, _lib.RB_E_SHAPE), q.shape[0], detail="out must have q's number of tokens")
+        import torch
+        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    _on(op, dev, q.dtype, out=out)
     return out
-
-
-def _stream_on(t, stream) -> int:
-    """The given stream, or the current one of t's device."""
-    import torch
-    return (stream if stream is not None else torch.cuda.current_stream(t.device)).cuda_stream
 
 
 # ----------------------------------------------------------------------------- codec surfaces

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "librocket_b200.so"
@@ -56,6 +57,13 @@ TILES_AUTO, TILES_SINGLE, TILES_PAIR = 0, 1, 2
 WEIGHT_I8G = 3
 WEIGHT_F16 = 4
 
+# Argument structures of the ragged-batch entry points, packed with the C
+# compiler's layout and passed as bytes: a third of the time of as many ctypes
+# arguments.
+KV_APPEND_ARGS = struct.Struct("3P3q2q2P4PqPq2P2qPq5if")
+ATTENTION_PAGED_ARGS = struct.Struct("2P2P4q2P2q2qP2q5i2f")
+ATTENTION_PACKED_ARGS = struct.Struct("3PP6qPq5i2f")
+
 SIGNATURES = {
     "rb_init": (_i, [_i]),
     "rb_last_error": (_i, [C.c_char_p, C.c_size_t]),
@@ -72,12 +80,9 @@ SIGNATURES = {
     "rb_pack_f32_q8_0_device": (_i64, [C.POINTER(_p), C.POINTER(_i64), _i, _i64]),
     "rb_attention_batched": (_i, [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _i, _i64, _i64, _i64, _i, _i, _i, _f, _f,
                                   _i, _i64, _i64, _i64, _p]),
-    "rb_kv_append": (_i, [_p, _i64, _p, _i64, _p, _i64, _i, _i64, _i64, _p, _p, _i, _i, _i, _p, _p, _f, _p, _p, _i64,
-                          _p, _i64, _p, _p, _i64, _i64, _i, _p, _i64, _p]),
-    "rb_attention_paged": (_i, [_p, _i64, _p, _p, _i64, _i64, _i, _p, _i64, _p, _p, _i64, _i64, _i64, _i64, _p, _i64,
-                                _i, _i, _i, _i, _f, _f, _i64, _p]),
-    "rb_attention_packed": (_i, [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _i, _i64, _i64, _p, _i, _i, _i, _f, _f, _i,
-                                 _i64, _p]),
+    "rb_kv_append": (_i, [C.c_char_p, _p]),
+    "rb_attention_paged": (_i, [C.c_char_p, _p]),
+    "rb_attention_packed": (_i, [C.c_char_p, _p]),
     "rb_rms_norm": (_i, [_p, _i, _p, _f, _p, _i, _i64, _i64, _p]),
     "rb_pack_f32_w8a8_device": (_i64, [_p, _i64, _i64, _f, _f]),
     "rb_pack_i8": (_i64, [_p, _i64, _i64, _i64]),

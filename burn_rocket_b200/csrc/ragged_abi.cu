@@ -98,12 +98,11 @@ int most_keys(int64_t ld_table, int page_size) {
 
 }  // namespace
 
-extern "C" int rb_kv_append(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
-                            int dtype, int64_t tokens, int64_t batch, const int32_t* cu_q, const int32_t* kv_len,
-                            int n_head, int n_kv_heads, int head_dim, const float* q_norm_w, const float* k_norm_w,
-                            float eps, const float* cos_t, const float* sin_t, int64_t max_pos, void* q_out,
-                            int64_t ldq_out, void* k_cache, void* v_cache, int64_t page_stride, int64_t num_pages,
-                            int page_size, const int32_t* page_table, int64_t ld_table, void* stream) {
+extern "C" int rb_kv_append(const rb_kv_append_args* args, void* stream) {
+  if (!args) return report_error(RB_E_SHAPE, "kv_append: null arguments");
+  const auto [q, k, v, ldq, ldk, ldv, tokens, batch, cu_q, kv_len, q_norm_w, k_norm_w, cos_t, sin_t, max_pos, q_out,
+              ldq_out, k_cache, v_cache, page_stride, num_pages, page_table, ld_table, dtype, n_head, n_kv_heads,
+              head_dim, page_size, eps] = *args;
   const char* op = "kv_append";
   int rc;
   const Heads h{n_head, n_kv_heads, head_dim};
@@ -154,12 +153,10 @@ extern "C" int rb_kv_append(const void* q, int64_t ldq, const void* k, int64_t l
   return RB_OK;
 }
 
-extern "C" int rb_attention_paged(const void* q, int64_t ldq, const void* k_cache, const void* v_cache,
-                                  int64_t page_stride, int64_t num_pages, int page_size, const int32_t* page_table,
-                                  int64_t ld_table, const int32_t* cu_q, const int32_t* kv_len, int64_t batch,
-                                  int64_t tokens, int64_t max_q, int64_t max_kv, void* out, int64_t ldo, int dtype,
-                                  int n_head, int n_kv_heads, int head_dim, float scale, float softcap,
-                                  int64_t window, void* stream) {
+extern "C" int rb_attention_paged(const rb_attention_paged_args* args, void* stream) {
+  if (!args) return report_error(RB_E_SHAPE, "attention_paged: null arguments");
+  const auto [q, out, k_cache, v_cache, ldq, ldo, tokens, batch, cu_q, kv_len, max_q, max_kv, page_stride, num_pages,
+              page_table, ld_table, window, dtype, n_head, n_kv_heads, head_dim, page_size, scale, softcap] = *args;
   const char* op = "attention_paged";
   int rc;
   const Heads h{n_head, n_kv_heads, head_dim};
@@ -200,10 +197,10 @@ extern "C" int rb_attention_paged(const void* q, int64_t ldq, const void* k_cach
   return RB_OK;
 }
 
-extern "C" int rb_attention_packed(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
-                                   void* out, int64_t ldo, int dtype, int64_t batch, int64_t tokens,
-                                   const int32_t* cu_seqlens, int n_head, int n_kv_heads, int head_dim, float scale,
-                                   float softcap, int mask_mode, int64_t window, void* stream) {
+extern "C" int rb_attention_packed(const rb_attention_packed_args* args, void* stream) {
+  if (!args) return report_error(RB_E_SHAPE, "attention_packed: null arguments");
+  const auto [q, k, v, out, ldq, ldk, ldv, ldo, tokens, batch, cu_seqlens, window, dtype, n_head, n_kv_heads, head_dim,
+              mask_mode, scale, softcap] = *args;
   const char* op = "attention_packed";
   int rc;
   const Heads h{n_head, n_kv_heads, head_dim};

@@ -259,7 +259,8 @@ RB_API int rb_attention_batched(const void* q, int64_t ldq, const void* k, int64
  * id outside the cache is not followed (its keys and values read as zeros, its
  * tokens are not stored), and rb_check_device_errors reports bad-shape.
  *
- * The calls allocate nothing and share no workspace: they may run at the same
+ * Arguments are structures (many, and cheap to pass through a binding); every
+ * field is read before the call returns. The calls allocate nothing and share no workspace: they may run at the same
  * time on several streams and in several graphs. */
 
 /* Appends the new tokens of each sequence to the cache: token i of sequence b
@@ -270,12 +271,23 @@ RB_API int rb_attention_batched(const void* q, int64_t ldq, const void* k, int64
  * are f32 [max_pos, head_dim/2] as for rb_rope. Arithmetic in f32, one rounding.
  * q_out may be q itself (with ldq_out == ldq). Two tokens must not map to one
  * slot. */
-RB_API int rb_kv_append(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
-                        int dtype, int64_t tokens, int64_t batch, const int32_t* cu_q, const int32_t* kv_len,
-                        int n_head, int n_kv_heads, int head_dim, const float* q_norm_w, const float* k_norm_w,
-                        float eps, const float* cos, const float* sin, int64_t max_pos, void* q_out,
-                        int64_t ldq_out, void* k_cache, void* v_cache, int64_t page_stride, int64_t num_pages,
-                        int page_size, const int32_t* page_table, int64_t ld_table, void* stream);
+typedef struct rb_kv_append_args {
+  const void *q, *k, *v;
+  int64_t ldq, ldk, ldv; /* row strides in elements */
+  int64_t tokens, batch;
+  const int32_t *cu_q, *kv_len;
+  const float *q_norm_w, *k_norm_w, *cos, *sin;
+  int64_t max_pos;
+  void* q_out;
+  int64_t ldq_out;
+  void *k_cache, *v_cache;
+  int64_t page_stride, num_pages;
+  const int32_t* page_table;
+  int64_t ld_table;
+  int dtype, n_head, n_kv_heads, head_dim, page_size;
+  float eps;
+} rb_kv_append_args;
+RB_API int rb_kv_append(const rb_kv_append_args* args, void* stream);
 
 /* Causal grouped-query attention of each sequence's new tokens (1 for a
  * decode step, a chunk of a prompt, any mix) over its kv_len[b] cached
@@ -286,22 +298,36 @@ RB_API int rb_kv_append(const void* q, int64_t ldq, const void* k, int64_t ldk, 
  * rb_attention; scale must be positive. max_q bounds the new tokens of any
  * sequence; max_kv is the longest kv_len expected (0: the table's width): it
  * only guides how the work is divided. out must not be an input. */
-RB_API int rb_attention_paged(const void* q, int64_t ldq, const void* k_cache, const void* v_cache,
-                              int64_t page_stride, int64_t num_pages, int page_size, const int32_t* page_table,
-                              int64_t ld_table, const int32_t* cu_q, const int32_t* kv_len, int64_t batch,
-                              int64_t tokens, int64_t max_q, int64_t max_kv, void* out, int64_t ldo, int dtype,
-                              int n_head, int n_kv_heads, int head_dim, float scale, float softcap, int64_t window,
-                              void* stream);
+typedef struct rb_attention_paged_args {
+  const void* q;
+  void* out;
+  const void *k_cache, *v_cache;
+  int64_t ldq, ldo, tokens, batch;
+  const int32_t *cu_q, *kv_len;
+  int64_t max_q, max_kv;
+  int64_t page_stride, num_pages;
+  const int32_t* page_table;
+  int64_t ld_table, window;
+  int dtype, n_head, n_kv_heads, head_dim, page_size;
+  float scale, softcap;
+} rb_attention_paged_args;
+RB_API int rb_attention_paged(const rb_attention_paged_args* args, void* stream);
 
 /* Grouped-query attention within each of `batch` packed sequences (whole
  * prompts, images): q, k, v and out rows [cu_seqlens[b], cu_seqlens[b+1])
  * belong to sequence b. mask_mode is RB_MASK_NONE, CAUSAL, WINDOW or
  * CAUSAL_WINDOW (window < 0 = unwindowed), head_dim 64, 72 or 128; a query that
  * sees no key is zero, otherwise as rb_attention_paged. */
-RB_API int rb_attention_packed(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
-                               void* out, int64_t ldo, int dtype, int64_t batch, int64_t tokens,
-                               const int32_t* cu_seqlens, int n_head, int n_kv_heads, int head_dim, float scale,
-                               float softcap, int mask_mode, int64_t window, void* stream);
+typedef struct rb_attention_packed_args {
+  const void *q, *k, *v;
+  void* out;
+  int64_t ldq, ldk, ldv, ldo, tokens, batch;
+  const int32_t* cu_seqlens;
+  int64_t window;
+  int dtype, n_head, n_kv_heads, head_dim, mask_mode;
+  float scale, softcap;
+} rb_attention_packed_args;
+RB_API int rb_attention_packed(const rb_attention_packed_args* args, void* stream);
 
 /* ---- glue ops of the RocketOps surface (ext.rs:70-83, 1054-1152; formulas
  * host.rs:15-72). Device buffers, any float dtype, asynchronous on `stream`. */

@@ -12,18 +12,21 @@ def call(name, base, **change):
     args = dict(base)
     assert set(change) <= set(args), change
     args.update(change)
-    return getattr(_lib.load(), name)(*args.values())
+    packer = {"rb_kv_append": _lib.KV_APPEND_ARGS, "rb_attention_paged": _lib.ATTENTION_PAGED_ARGS,
+              "rb_attention_packed": _lib.ATTENTION_PACKED_ARGS}[name]
+    return getattr(_lib.load(), name)(packer.pack(*(0 if v is None else v for v in args.values())), None)
 
 
-APPEND = dict(q=P, ldq=2048, k=P + 64, ldk=1024, v=P + 128, ldv=1024, dtype=1, tokens=8, batch=2, cu=P, kv_len=P,
-              n_head=16, n_kv_heads=8, head_dim=128, q_norm=P, k_norm=None, eps=1e-6, cos=P, sin=P, max_pos=100,
-              q_out=P + 256, ldq_out=2048, k_cache=P, v_cache=P, page_stride=16 * 1024, num_pages=10, page_size=16,
-              table=P, ld_table=4, stream=None)
-PAGED = dict(q=P + 64, ldq=2048, k_cache=P, v_cache=P, page_stride=16 * 1024, num_pages=10, page_size=16, table=P,
-             ld_table=4, cu=P, kv_len=P, batch=2, tokens=8, max_q=4, max_kv=0, out=P + 256, ldo=2048, dtype=2,
-             n_head=16, n_kv_heads=8, head_dim=128, scale=0.1, softcap=0.0, window=-1, stream=None)
-PACKED = dict(q=P, ldq=4096, k=P + 64, ldk=4096, v=P + 128, ldv=4096, out=P + 256, ldo=2048, dtype=1, batch=2, tokens=8,
-              cu=P, n_head=16, n_kv_heads=8, head_dim=128, scale=0.1, softcap=0.0, mode=2, window=-1, stream=None)
+# In the order of the C structures.
+APPEND = dict(q=P, k=P + 64, v=P + 128, ldq=2048, ldk=1024, ldv=1024, tokens=8, batch=2, cu=P, kv_len=P, q_norm=P,
+              k_norm=None, cos=P, sin=P, max_pos=100, q_out=P + 256, ldq_out=2048, k_cache=P, v_cache=P,
+              page_stride=16 * 1024, num_pages=10, table=P, ld_table=4, dtype=1, n_head=16, n_kv_heads=8, head_dim=128,
+              page_size=16, eps=1e-6)
+PAGED = dict(q=P + 64, out=P + 256, k_cache=P, v_cache=P, ldq=2048, ldo=2048, tokens=8, batch=2, cu=P, kv_len=P, max_q=4,
+             max_kv=0, page_stride=16 * 1024, num_pages=10, table=P, ld_table=4, window=-1, dtype=2, n_head=16,
+             n_kv_heads=8, head_dim=128, page_size=16, scale=0.1, softcap=0.0)
+PACKED = dict(q=P, k=P + 64, v=P + 128, out=P + 256, ldq=4096, ldk=4096, ldv=4096, ldo=2048, tokens=8, batch=2, cu=P,
+              window=-1, dtype=1, n_head=16, n_kv_heads=8, head_dim=128, mode=2, scale=0.1, softcap=0.0)
 NAN, INF = float("nan"), float("inf")
 
 COMMON = [dict(dtype=0), dict(dtype=3), dict(tokens=-1), dict(batch=-1), dict(tokens=1 << 31), dict(n_head=15),
@@ -39,7 +42,7 @@ SOFTMAX = [dict(scale=0.0), dict(scale=-0.1), dict(scale=NAN), dict(scale=INF), 
 @pytest.mark.parametrize("change", COMMON + CACHE + [
     dict(q=None), dict(k=None), dict(v=None), dict(q_out=None), dict(ldq=2040), dict(ldk=1020), dict(ldv=1028),
     dict(q=P + 8), dict(k=P + 2), dict(q_out=P + 4), dict(cos=None), dict(sin=None), dict(cos=P + 4), dict(q_norm=P + 8),
-    dict(max_pos=0), dict(eps=NAN), dict(eps=-1.0), dict(q_out=P, ldq=4096)])
+    dict(max_pos=0), dict(eps=NAN), dict(eps=-1.0), dict(q_out=P, ldq=4096)])  # in place with two strides
 def test_kv_append_refuses(change):
     rc = call("rb_kv_append", APPEND, **change)
     assert rc in (_lib.RB_E_SHAPE, _lib.RB_E_UNSUPPORTED), (rc, change)
@@ -70,6 +73,29 @@ def test_attention_packed_refuses(change):
 def test_empty_batches_are_no_work(name, base):
     assert call(name, base, tokens=0) == _lib.RB_OK
     assert call(name, base, batch=0) == _lib.RB_OK
+
+
+def test_argument_structures_match_the_header(tmp_path):
+    """The packed layouts are the C compiler's."""
+    import subprocess
+    import struct
+    from pathlib import Path
+    header = Path(__file__).resolve().parent.parent / "include" / "rocket_b200.h"
+    src = tmp_path / "layout.c"
+    src.write_text(f'''#include <stdio.h>
+#include <stddef.h>
+#include "{header}"
+int main(void) {{
+  printf("%zu %zu %zu\\n", sizeof(rb_kv_append_args), sizeof(rb_attention_paged_args), sizeof(rb_attention_packed_args));
+  printf("%zu %zu %zu\\n", offsetof(rb_kv_append_args, eps), offsetof(rb_attention_paged_args, softcap),
+         offsetof(rb_attention_packed_args, softcap));
+}}''')
+    subprocess.run(["gcc", str(src), "-o", str(tmp_path / "layout")], check=True)
+    sizes, last = subprocess.run([str(tmp_path / "layout")], check=True, capture_output=True, text=True).stdout.splitlines()
+    packers = (_lib.KV_APPEND_ARGS, _lib.ATTENTION_PAGED_ARGS, _lib.ATTENTION_PACKED_ARGS)
+    assert [p.size - 4 for p in packers] == [int(x) for x in last.split()]
+    assert [(p.size + 7) // 8 * 8 for p in packers] == [int(x) for x in sizes.split()]
+    assert struct.calcsize("P") == 8
 
 
 def test_good_arguments_need_the_engine():
