@@ -19,10 +19,9 @@
 // computed again from the definition (row_attention).
 //
 // Schedules:
-//   * persistent: a CTA an SM walks the units heaviest first (unit level t = its
-//     tile's index in the sequence, found by counting how many units lie at or
-//     above a level), the next unit's Q and first tiles loading while this one
-//     finishes;
+//   * persistent: a CTA an SM walks units ranked by cost, heaviest first and back
+//     and forth over the CTAs, the next unit's Q and first tiles loading while
+//     this one finishes;
 //   * split: where there are fewer units than SMs, a cluster of CTAs takes equal
 //     runs of one unit's key tiles and merges (O, m, l) through distributed
 //     shared memory: no workspace in global memory.
@@ -150,53 +149,131 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
   return v;
 }
 
-// The unit of rank r (one warp): units are ordered by level, highest first, and
-// by sequence within a level; sequence b has levels 0 .. ceil(n_b / (2 tq)) - 1.
-// False past the last unit.
-__device__ __forceinline__ bool find_unit(const TileParams& p, int r, int& b, int& level) {
-  const int lane = threadIdx.x & 31, batch = p.a.seqs.batch, span = 2 * p.tq;
-  auto levels = [&](int s) { return s < batch ? (load_seq(p.a.seqs, s).n + span - 1) / span : 0; };
-  const int own = levels(lane);  // the first 32 sequences stay in registers
-  auto at_or_above = [&](int t) {
-    int c = max(0, own - t);
-    for (int s = 32 + lane; s < batch; s += 32) c += max(0, levels(s) - t);
-    return static_cast<int>(__reduce_add_sync(0xffffffffu, c));
+// Among each four lanes: lane i's chunk e and lane e's chunk i change places.
+__device__ __forceinline__ void transpose4(uint4 (&w)[4], int lane) {
+  auto swap = [](uint4& a, uint4& b, bool upper, int mask) {  // the lower lane's b with the upper lane's a
+    uint4 s = upper ? a : b;
+    s.x = __shfl_xor_sync(0xffffffffu, s.x, mask);
+    s.y = __shfl_xor_sync(0xffffffffu, s.y, mask);
+    s.z = __shfl_xor_sync(0xffffffffu, s.z, mask);
+    s.w = __shfl_xor_sync(0xffffffffu, s.w, mask);
+    if (upper) a = s;
+    else b = s;
   };
-  int top = own;
-  for (int s = 32 + lane; s < batch; s += 32) top = max(top, levels(s));
-  top = __reduce_max_sync(0xffffffffu, top);
-  if (top == 0 || at_or_above(0) <= r) return false;
-  int lo = 0, hi = top;  // at_or_above(lo) > r >= at_or_above(hi) = 0
-  int above = 0;         // at_or_above(hi)
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2, c = at_or_above(mid);
-    if (c > r) lo = mid;
-    else hi = mid, above = c;
-  }
-  level = lo;
-  int idx = r - above;  // among the sequences with more than `level` levels
-  for (int s0 = 0; s0 < batch; s0 += 32) {
-    const unsigned m = __ballot_sync(0xffffffffu, (s0 == 0 ? own : levels(s0 + lane)) > level);
-    const int c = __popc(m);
-    if (idx < c) {
-      b = s0 + __fns(m, 0, idx + 1);
-      return true;
-    }
-    idx -= c;
-  }
-  return false;
+  swap(w[0], w[1], lane & 1, 1);
+  swap(w[2], w[3], lane & 1, 1);
+  swap(w[0], w[2], lane & 2, 2);
+  swap(w[1], w[3], lane & 2, 2);
 }
 
+// Where a unit lies (one warp). A sequence has L = ceil(n / span) spans of
+// span = 2 tq tokens; span t of sequence b costs F + t + 1 (in spans of keys,
+// F = floor(first position / span)) when causal and L otherwise. Up to 128
+// sequences are held in registers, four a lane, and units are ranked by cost,
+// highest first: the units of cost >= T are counted in closed form, and the T
+// of rank r is found by bisection. Larger batches take their units in order.
+struct Finder {
+  int L[4], F[4], q0[4], n[4], kv[4];
+  int total, top;   // ranked: units, and the highest cost
+  int seq, before;  // in order: a sequence and the units before it
+  bool causal, ranked;
+
+  __device__ __forceinline__ Seq fetch(const TileParams& p, int b) const {
+    return b < p.a.seqs.batch ? load_seq(p.a.seqs, b) : Seq{0, 0, 0};
+  }
+  __device__ __forceinline__ void init(const TileParams& p) {
+    const int lane = threadIdx.x & 31, span = 2 * p.tq;
+    causal = p.a.dhi == 0;
+    ranked = p.a.seqs.batch <= 128;
+    seq = before = total = top = 0;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const Seq s = ranked ? fetch(p, 32 * g + lane) : Seq{0, 0, 0};
+      q0[g] = s.q0;
+      n[g] = s.n;
+      kv[g] = s.kv;
+      L[g] = (s.n + span - 1) / span;
+      F[g] = causal ? max(0, s.kv - s.n) / span : 0;
+      total += L[g];
+      top = max(top, L[g] ? L[g] + F[g] : 0);
+    }
+    total = __reduce_add_sync(0xffffffffu, total);
+    top = __reduce_max_sync(0xffffffffu, top);
+  }
+  __device__ __forceinline__ int at_least(int g, int T) const {  // units of cost >= T of the lane's sequence g
+    return causal ? max(0, L[g] - max(0, T - 1 - F[g])) : (L[g] >= T ? L[g] : 0);
+  }
+  __device__ __forceinline__ int count(int T) const {
+    return __reduce_add_sync(0xffffffffu, at_least(0, T) + at_least(1, T) + at_least(2, T) + at_least(3, T));
+  }
+  __device__ __forceinline__ bool find(const TileParams& p, int r, int& b, int& t, Seq& s) {
+    const int lane = threadIdx.x & 31, span = 2 * p.tq;
+    if (!ranked) {
+      if (r < before) seq = before = 0;
+      while (seq < p.a.seqs.batch) {
+        const Seq x = fetch(p, seq + lane);
+        const int own = (x.n + span - 1) / span;
+        int sum = own;  // inclusive prefix
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, sum, o);
+          if (lane >= o) sum += y;
+        }
+        const int all = __shfl_sync(0xffffffffu, sum, 31);
+        if (r < before + all) {
+          const int at = __ffs(__ballot_sync(0xffffffffu, r < before + sum)) - 1;
+          b = seq + at;
+          t = r - before - __shfl_sync(0xffffffffu, sum - own, at);
+          s = Seq{__shfl_sync(0xffffffffu, x.q0, at), __shfl_sync(0xffffffffu, x.n, at),
+                  __shfl_sync(0xffffffffu, x.kv, at)};
+          return true;
+        }
+        before += all;
+        seq += 32;
+      }
+      return false;
+    }
+    if (r >= total) return false;
+    int lo = 1, hi = top + 1, above = 0;  // count(lo) > r >= count(hi) = above
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2, c = count(mid);
+      if (c > r) lo = mid;
+      else hi = mid, above = c;
+    }
+    int idx = r - above;  // among the units of cost lo
+    if (!causal) {
+      t = idx % lo;
+      idx /= lo;
+    }
+    bool found = false;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const unsigned m = __ballot_sync(0xffffffffu, at_least(g, lo) > at_least(g, lo + 1));
+      const int c = __popc(m), at = !found && idx < c ? __fns(m, 0, idx + 1) : 0;
+      const int f = __shfl_sync(0xffffffffu, F[g], at), a = __shfl_sync(0xffffffffu, q0[g], at);
+      const int d = __shfl_sync(0xffffffffu, n[g], at), e = __shfl_sync(0xffffffffu, kv[g], at);
+      if (!found && idx < c) {
+        found = true;
+        b = 32 * g + at;
+        if (causal) t = lo - 1 - f;
+        s = Seq{a, d, e};
+      }
+      idx -= c;
+    }
+    return found;
+  }
+};
+
 // One warp: the item of unit u, this CTA being `rank` of `ranks`.
-__device__ __forceinline__ Item make_item(const TileParams& p, int u, int rank, int ranks) {
+__device__ __forceinline__ Item make_item(const TileParams& p, Finder& f, int u, int rank, int ranks) {
   Item it;
+  Seq s;
   int level;
   it.b = -1;
-  if (u < 0 || !find_unit(p, u / p.a.n_kv_heads, it.b, level)) {
+  if (u < 0 || !f.find(p, u / p.a.n_kv_heads, it.b, level, s)) {
     it.b = -1;
     return it;
   }
-  const Seq s = load_seq(p.a.seqs, it.b);
   it.q0 = s.q0;
   it.n = s.n;
   it.kv = s.kv;
@@ -312,8 +389,10 @@ tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
     const int page = kv.table ? 1 << kv.page_shift : 0;
     const int per_tile = kv.table ? BN >> kv.page_shift : 0;  // pages a tile
     int kv_base = 0, loaded = 0;
+    Finder finder;
+    finder.init(p);
     for (int k = 0;; ++k) {
-      const Item it = make_item(p, unit_of(k), rank, ranks);
+      const Item it = make_item(p, finder, unit_of(k), rank, ranks);
       if (k >= 2 && !warp_wait(&i_empty[k & 1], ((k >> 1) - 1) & 1, err, abort_flag)) break;
       if (lane == 0) {
         items[k & 1] = it;
@@ -544,22 +623,25 @@ tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
         const int ka = j * BN;
         const bool inner = ka >= all_lo && ka + BN - 1 <= all_hi;
         const int vlo = max(row_lo - ka, 0), vhi = min(row_hi - ka, BN - 1);
-        float mraw;
-        if (inner) {
-          float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
+        if (!inner) {  // one mask word per 32 columns
 #pragma unroll
-          for (int e = 0; e < BN; e += 8) {
-            m0 = max3n(m0, x[e], x[e + 1]);
-            m1 = max3n(m1, x[e + 2], x[e + 3]);
-            m2 = max3n(m2, x[e + 4], x[e + 5]);
-            m3 = max3n(m3, x[e + 6], x[e + 7]);
+          for (int c0 = 0; c0 < BN; c0 += 32) {
+            const int a = min(max(vlo - c0, 0), 32), z = min(max(vhi + 1 - c0, 0), 32);  // columns [a, z)
+            const uint32_t up = z == 32 ? 0xffffffffu : (1u << z) - 1u, down = a == 32 ? 0xffffffffu : (1u << a) - 1u;
+            const uint32_t mask = up & ~down;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) x[c0 + e] = (mask >> e & 1u) ? x[c0 + e] : -INFINITY;
           }
-          mraw = max2n(max2n(m0, m1), max2n(m2, m3));
-        } else {
-          mraw = -INFINITY;
-#pragma unroll
-          for (int e = 0; e < BN; ++e) mraw = max2n(mraw, (e >= vlo && e <= vhi) ? x[e] : -INFINITY);
         }
+        float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < BN; e += 8) {
+          m0 = max3n(m0, x[e], x[e + 1]);
+          m1 = max3n(m1, x[e + 2], x[e + 3]);
+          m2 = max3n(m2, x[e + 4], x[e + 5]);
+          m3 = max3n(m3, x[e + 6], x[e + 7]);
+        }
+        const float mraw = max2n(max2n(m0, m1), max2n(m2, m3));
         const float c = p.a.scale * kLog2e, mt = mraw * c;
         float alpha = 1.0f;
         bool need = false;
@@ -570,18 +652,19 @@ tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
           m_used = mt;
           need = true;
         }
-        const float nm = -m_used;
+        const float nm = m_used == -INFINITY ? 0.0f : -m_used;  // nothing visible yet: weights are 0
         uint64_t rs[2] = {0ull, 0ull};
 #pragma unroll
         for (int c0 = 0; c0 < BN; c0 += 32) {
           uint32_t pk[16];
-          if (inner) {
-            const uint64_t c2 = f2_pack(c, c), nm2 = f2_pack(nm, nm);
+          const uint64_t c2 = f2_pack(c, c), nm2 = f2_pack(nm, nm);
+          // (The polynomial floors at 2^-126, where a masked score must give 0.)
+          if (D >= 128 && inner) {
 #pragma unroll
             for (int e = 0; e < 32; e += 2) {
               float y0, y1, p0, p1;
               f2_unpack(f2_fma(f2_pack(x[c0 + e], x[c0 + e + 1]), c2, nm2), y0, y1);
-              if (D >= 128 && (e / 2) % 4 == 3) {
+              if ((e / 2) % 4 == 3) {
                 exp2_poly2(y0, y1, p0, p1);
               } else {
                 p0 = ex2(y0);
@@ -593,10 +676,9 @@ tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
           } else {
 #pragma unroll
             for (int e = 0; e < 32; e += 2) {
-              const int k0 = c0 + e;
-              float p0 = ex2(fmaf(x[k0], c, nm)), p1 = ex2(fmaf(x[k0 + 1], c, nm));
-              p0 = (k0 >= vlo && k0 <= vhi) ? p0 : 0.0f;
-              p1 = (k0 + 1 >= vlo && k0 + 1 <= vhi) ? p1 : 0.0f;
+              float y0, y1;
+              f2_unpack(f2_fma(f2_pack(x[c0 + e], x[c0 + e + 1]), c2, nm2), y0, y1);
+              const float p0 = ex2(y0), p1 = ex2(y1);
               rs[(e / 2) & 1] = f2_add(rs[(e / 2) & 1], f2_pack(p0, p1));
               pk[e / 2] = pack2<BF16>(p0, p1);
             }
@@ -672,6 +754,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
         continue;
       }
       const bool empty = row_lo > row_hi;
+      const unsigned valid_rows = __ballot_sync(0xffffffffu, valid);
       const float inv = 1.0f / l;
       float check = 0.0f;
 #pragma unroll
@@ -684,19 +767,35 @@ tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
           __syncwarp();
           if (lane == 0) mbar_arrive(&o_free[s]);
         }
+        uint4 w[4];
 #pragma unroll
-        for (int e = 0; e < 32; e += 8) {
-          if (c0 + e >= DH) continue;
-          uint32_t w[4];
+        for (int e = 0; e < 4; ++e) {
+          uint32_t u[4];
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            const float y0 = __uint_as_float(r[e + 2 * q]) * inv, y1 = __uint_as_float(r[e + 2 * q + 1]) * inv;
-            check = fmaf(y0, 0.0f, fmaf(y1, 0.0f, check));
-            w[q] = empty ? 0u : pack2<BF16>(y0, y1);
+            const float y0 = __uint_as_float(r[8 * e + 2 * q]) * inv, y1 = __uint_as_float(r[8 * e + 2 * q + 1]) * inv;
+            if (c0 + 8 * e < DH) check = fmaf(y0, 0.0f, fmaf(y1, 0.0f, check));
+            u[q] = empty ? 0u : pack2<BF16>(y0, y1);
           }
-          if (valid) reinterpret_cast<uint4*>(out + c0 + e)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+          w[e] = make_uint4(u[0], u[1], u[2], u[3]);
+        }
+        if (c0 + 32 <= DH) {
+          // Four lanes turn their four chunks about, so that one store covers
+          // 64 contiguous bytes of eight rows instead of 16 of thirty-two.
+          transpose4(w, lane);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int from = (lane & ~3) + e;
+            uint16_t* dst = reinterpret_cast<uint16_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(out), from));
+            if (valid_rows >> from & 1) *reinterpret_cast<uint4*>(dst + c0 + 8 * (lane & 3)) = w[e];
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (valid && c0 + 8 * e < DH) *reinterpret_cast<uint4*>(out + c0 + 8 * e) = w[e];
         }
       }
+      __syncwarp();  // before the mark: other lanes stored parts of the row
       if (valid && !empty && !(check == 0.0f)) {  // marked by a NaN of either type
         *reinterpret_cast<uint32_t*>(out) = 0x7fff7fffu;
         redo[0] = 1;
@@ -737,8 +836,10 @@ tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
   }
   if (!SPLIT && redo[0] && !*abort_flag) {  // (redo is read after the barrier above)
     // The marked rows of this CTA's units, again from the definition.
+    Finder finder;
+    finder.init(p);
     for (int k = 0;; ++k) {
-      const Item it = make_item(p, unit_of(k), 0, 1);
+      const Item it = make_item(p, finder, unit_of(k), 0, 1);
       if (it.b < 0) break;
       for (int rr = warp; rr < 2 * p.tq * p.group; rr += kThreads / 32) {
         const int i = it.i0 + rr / p.group, head = it.g * p.group + rr % p.group;
