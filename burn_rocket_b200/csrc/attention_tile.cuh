@@ -6,7 +6,7 @@
 // share the KV head, so a key tile is loaded once for every head that reads it
 // and a short run of tokens still fills rows. Warp 0 finds units and feeds TMA (Q
 // per unit, K and V rings of 128-key tiles; from a paged cache one box a page),
-// warp 1 issues UMMAs, warps 2-5 and 6-9 are the softmax of slot 0 and 1, one row
+// warp 1 issues UMMAs, warps 4-7 and 8-11 are the softmax of slot 0 and 1, one row
 // a thread. Per slot TMEM holds S (128 x 128 f32, P written over it as 16-bit)
 // and O; the two slots alternate on the tensor pipe, S(j+1) following P·V(j).
 //
@@ -38,8 +38,14 @@ namespace tile {
 
 constexpr int BM = 128;  // rows of a slot
 constexpr int BN = 128;  // keys of a tile
-constexpr int kThreads = 10 * 32;
-constexpr int kSoftWarp0 = 2;
+// Three warpgroups: warps 0-3 (TMA, UMMA, two idle), 4-7 and 8-11 (softmax of
+// slot 0 and 1). The block starts with kLaunchRegs a thread; the first warpgroup
+// hands registers to the other two, whose 128 scores a row do not fit 168.
+constexpr int kThreads = 12 * 32;
+constexpr int kSoftWarp0 = 4;
+constexpr int kSoftThreads = 8 * 32;
+constexpr int kLaunchRegs = 168, kRoleRegs = 104, kSoftRegs = 200;
+static_assert(kRoleRegs + 2 * kSoftRegs <= 3 * kLaunchRegs, "the shares come from the launch's registers");
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescale = 8.0f;  // log2 units
 
@@ -102,24 +108,6 @@ __device__ __forceinline__ float max3n(float a, float b, float c) {
   return d;
 }
 
-// 2^y of a pair on the FMA pipe (the dense kernel's polynomial: range
-// reduction by 1.5 * 2^23 rounded down, degree 3, 7.5e-5 relative).
-__device__ __forceinline__ void exp2_poly2(float y0, float y1, float& p0, float& p1) {
-  const uint64_t y = f2_pack(fmaxf(y0, -126.0f), fmaxf(y1, -126.0f));
-  const uint64_t t = f2_add_rm(y, f2_pack(12582912.0f, 12582912.0f));
-  const uint64_t j = f2_add(t, f2_pack(-12582912.0f, -12582912.0f));
-  const uint64_t f = f2_fma(j, f2_pack(-1.0f, -1.0f), y);
-  uint64_t q = f2_fma(f2_pack(0.07802403173175049f, 0.07802403173175049f), f,
-                      f2_pack(0.22606706619262695f, 0.22606706619262695f));
-  q = f2_fma(q, f, f2_pack(0.6958339810371399f, 0.6958339810371399f));
-  q = f2_fma(q, f, f2_pack(0.9999251365661621f, 0.9999251365661621f));
-  float q0, q1, t0, t1;
-  f2_unpack(q, q0, q1);
-  f2_unpack(t, t0, t1);
-  p0 = __uint_as_float(__float_as_uint(q0) + (__float_as_uint(t0) << 23));
-  p1 = __uint_as_float(__float_as_uint(q1) + (__float_as_uint(t1) << 23));
-}
-
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   if (BF16) {
@@ -147,6 +135,11 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
                : "r"(addr)
                : "memory");
   return v;
+}
+
+// The softmax warps among themselves.
+__device__ __forceinline__ void soft_sync() {
+  asm volatile("barrier.cta.sync 1, %0;" ::"n"(kSoftThreads) : "memory");
 }
 
 // Among each four lanes: lane i's chunk e and lane e's chunk i change places.
@@ -325,11 +318,12 @@ tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
   uint64_t* o_free = o_done + 2;       // [slot] the unit's O was read out
   uint64_t* i_full = o_free + 2;       // [2] an item is there
   uint64_t* i_empty = i_full + 2;      // [2] every role has read it
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(i_empty + 2);
+  uint64_t* turns = i_empty + 2;       // [lane quarter][slot] whose exponentials run
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(turns + 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   uint32_t* redo = tmem_slot + 2;      // [8] rows to compute again (one a bit when split, else a flag)
   Item* items = reinterpret_cast<Item*>(redo + 8);  // [2]
-  static_assert((2 + 2 * KS + 2 * VS + 12) * 8 + 48 + 2 * sizeof(Item) <= 1024, "barrier area");
+  static_assert((2 + 2 * KS + 2 * VS + 20) * 8 + 48 + 2 * sizeof(Item) <= 1024, "barrier area");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t* err = p.a.seqs.err;
@@ -348,6 +342,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
       mbar_init(&i_full[i], 1);
       mbar_init(&i_empty[i], 9);
     }
+    for (int i = 0; i < 8; ++i) mbar_init(&turns[i], 1);
     *abort_flag = 0;
     for (int i = 0; i < 8; ++i) redo[i] = 0;
     fence_mbar_init();
@@ -374,9 +369,9 @@ tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
     return true;
   };
 
-  float part_m = -INFINITY, part_l = 0.0f;  // split: a softmax thread's row of this CTA's run
-  bool part_o = false;
-
+  if (warp < kSoftWarp0) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRoleRegs));
+  }
   if (warp == 0) {
     // ------------------------------------------------------------ units and TMA
     if (lane == 0) {
@@ -569,14 +564,42 @@ tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
         kv_base += it.jb - it.ja + 1;
       }
     }
+  }
+  if (warp < kSoftWarp0) {
+    tc_fence_before();
+    __syncthreads();
+    if (*abort_flag) drain_after_abort();
+    if (SPLIT) __syncthreads();  // the partials are out of TMEM
+    if (warp == 1) {
+      tc_fence_after();
+      tmem_dealloc(tmem_base, 512);
+    }
+    if (SPLIT) {
+      cluster_sync_all();
+      cluster_sync_all();
+    }
   } else {
     // ------------------------------------------------------------ softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
+    float part_m = -INFINITY, part_l = 0.0f;  // split: this thread's row of the CTA's run
+    bool part_o = false;
     const int s = (warp - kSoftWarp0) >> 2;
     const int row = (warp & 3) * 32 + lane;  // TMEM lane
     const uint32_t lane_base = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t s_col = s * 256, o_col = s * 256 + 128;
     const int tok = row / p.group, sub = row - tok * p.group;
     int it_n = 0, kv_base = 0;
+    // The warp of the other slot on the same lanes sits on the same
+    // sub-partition: they take turns, tile by tile, at the exponentials, slot 0
+    // first. Left alone both slots run them together at half the MUFU's rate
+    // each and then wait for the tensor pipe together.
+    uint64_t* my_turn = &turns[(warp & 3) * 2 + s];
+    uint64_t* its_turn = &turns[(warp & 3) * 2 + (s ^ 1)];
+    int n_turn = 0;
+    if (s == 1 && lane == 0) mbar_arrive(its_turn);
+    auto take_turn = [&]() -> bool {
+      return __all_sync(0xffffffffu, mbar_wait(my_turn, n_turn++ & 1, err, abort_flag));
+    };
     Item it;
     for (int k = 0;; ++k) {
       if (!__all_sync(0xffffffffu, get_item(k, it))) break;
@@ -594,8 +617,13 @@ tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
       visible(first_pos + min(it.n, ia + p.tq) - 1, it.kv, p.a.dlo, p.a.dhi, all_lo, x0);
       float m_used = -INFINITY, l = 0.0f;
       bool ok = true;
-      for (int j = lo; j <= hi; ++j, ++it_n) {
-        if (!__all_sync(0xffffffffu, mbar_wait(&s_full[s], it_n & 1, err, abort_flag))) {
+      for (int j = it.ja; ok && j <= it.jb; ++j) {
+        if (j < lo || j > hi) {  // the other slot's tile: pass the turn on
+          ok = take_turn();
+          if (lane == 0) mbar_arrive(its_turn);
+          continue;
+        }
+        if (!__all_sync(0xffffffffu, mbar_wait(&s_full[s], it_n++ & 1, err, abort_flag))) {
           ok = false;
           break;
         }
@@ -653,38 +681,23 @@ tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
           need = true;
         }
         const float nm = m_used == -INFINITY ? 0.0f : -m_used;  // nothing visible yet: weights are 0
+        if (!(ok = take_turn())) break;
         uint64_t rs[2] = {0ull, 0ull};
 #pragma unroll
         for (int c0 = 0; c0 < BN; c0 += 32) {
           uint32_t pk[16];
           const uint64_t c2 = f2_pack(c, c), nm2 = f2_pack(nm, nm);
-          // (The polynomial floors at 2^-126, where a masked score must give 0.)
-          if (D >= 128 && inner) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              float y0, y1, p0, p1;
-              f2_unpack(f2_fma(f2_pack(x[c0 + e], x[c0 + e + 1]), c2, nm2), y0, y1);
-              if ((e / 2) % 4 == 3) {
-                exp2_poly2(y0, y1, p0, p1);
-              } else {
-                p0 = ex2(y0);
-                p1 = ex2(y1);
-              }
-              rs[(e / 2) & 1] = f2_add(rs[(e / 2) & 1], f2_pack(p0, p1));
-              pk[e / 2] = pack2<BF16>(p0, p1);
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              float y0, y1;
-              f2_unpack(f2_fma(f2_pack(x[c0 + e], x[c0 + e + 1]), c2, nm2), y0, y1);
-              const float p0 = ex2(y0), p1 = ex2(y1);
-              rs[(e / 2) & 1] = f2_add(rs[(e / 2) & 1], f2_pack(p0, p1));
-              pk[e / 2] = pack2<BF16>(p0, p1);
-            }
+          for (int e = 0; e < 32; e += 2) {
+            float y0, y1;
+            f2_unpack(f2_fma(f2_pack(x[c0 + e], x[c0 + e + 1]), c2, nm2), y0, y1);
+            const float p0 = ex2(y0), p1 = ex2(y1);
+            rs[(e / 2) & 1] = f2_add(rs[(e / 2) & 1], f2_pack(p0, p1));
+            pk[e / 2] = pack2<BF16>(p0, p1);
           }
           tmem_st16(lane_base + s_col + c0 / 2, pk);
         }
+        if (lane == 0) mbar_arrive(its_turn);
         float a0, a1, a2, a3;
         f2_unpack(rs[0], a0, a1);
         f2_unpack(rs[1], a2, a3);
@@ -801,120 +814,115 @@ tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
         redo[0] = 1;
       }
     }
-  }
 
-  tc_fence_before();
-  __syncthreads();
-  if (*abort_flag) drain_after_abort();
-  if (SPLIT && warp >= kSoftWarp0) {  // the rings are idle: they take the partials
-    tc_fence_after();
-    const int s = (warp - kSoftWarp0) >> 2, row = (warp & 3) * 32 + lane;
-    float4* part = reinterpret_cast<float4*>(smem + s * L::PART);
-    float* stat = reinterpret_cast<float*>(smem + 2 * L::PART) + s * 2 * BM;
-    if (__any_sync(0xffffffffu, part_o)) {
-      const uint32_t o = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16) + s * 256 + 128;
-#pragma unroll
-      for (int c0 = 0; c0 < D; c0 += 32) {
-        uint32_t r[32];
-        tmem_ld32(o + c0, r);
-        tmem_wait_ld();
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (c0 + 4 * e < D)
-            part[(c0 / 4 + e) * BM + row] = make_float4(__uint_as_float(r[4 * e]), __uint_as_float(r[4 * e + 1]),
-                                                        __uint_as_float(r[4 * e + 2]), __uint_as_float(r[4 * e + 3]));
-      }
-    }
-    stat[row] = part_m;
-    stat[BM + row] = part_l;
     tc_fence_before();
-  }
-  if (SPLIT) __syncthreads();
-  if (warp == 1) {
-    tc_fence_after();
-    tmem_dealloc(tmem_base, 512);
-  }
-  if (!SPLIT && redo[0] && !*abort_flag) {  // (redo is read after the barrier above)
-    // The marked rows of this CTA's units, again from the definition.
-    Finder finder;
-    finder.init(p);
-    for (int k = 0;; ++k) {
-      const Item it = make_item(p, finder, unit_of(k), 0, 1);
-      if (it.b < 0) break;
-      for (int rr = warp; rr < 2 * p.tq * p.group; rr += kThreads / 32) {
-        const int i = it.i0 + rr / p.group, head = it.g * p.group + rr % p.group;
-        if (i >= it.n) break;
-        const uint16_t mark = p.a.out[static_cast<int64_t>(it.q0 + i) * p.a.ldo + head * DH];
-        if ((mark & 0x7fffu) != 0x7fffu) continue;
-        const Seq seq{it.q0, it.n, it.kv};
-        if (p.a.kv.table) row_attention<DH, BF16, true>(p.a, it.b, seq, i, head);
-        else row_attention<DH, BF16, false>(p.a, it.b, seq, i, head);
+    __syncthreads();
+    if (*abort_flag) drain_after_abort();
+    if (SPLIT) {  // the rings are idle: they take the partials
+      tc_fence_after();
+      float4* part = reinterpret_cast<float4*>(smem + s * L::PART);
+      float* stat = reinterpret_cast<float*>(smem + 2 * L::PART) + s * 2 * BM;
+      if (__any_sync(0xffffffffu, part_o)) {
+        const uint32_t o = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16) + s * 256 + 128;
+  #pragma unroll
+        for (int c0 = 0; c0 < D; c0 += 32) {
+          uint32_t r[32];
+          tmem_ld32(o + c0, r);
+          tmem_wait_ld();
+  #pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (c0 + 4 * e < D)
+              part[(c0 / 4 + e) * BM + row] = make_float4(__uint_as_float(r[4 * e]), __uint_as_float(r[4 * e + 1]),
+                                                          __uint_as_float(r[4 * e + 2]), __uint_as_float(r[4 * e + 3]));
+        }
       }
+      stat[row] = part_m;
+      stat[BM + row] = part_l;
+      tc_fence_before();
     }
-  }
-  if (SPLIT) {
-    cluster_sync_all();  // every partial is written
-    const Item it = items[0];
-    if (it.b >= 0 && !*abort_flag) {
-      const float* stat = reinterpret_cast<const float*>(smem + 2 * L::PART);       // [slot][m, l][BM]
-      float* all = reinterpret_cast<float*>(smem + 2 * L::PART) + 4 * BM;           // [rank][slot][m, l][rows]
-      // Rank k finishes the rows [k, k + 1) * 2 BM / ranks.
-      const int share = 2 * BM / ranks, r0 = rank * share;
-      for (int e = threadIdx.x; e < ranks * 2 * share; e += kThreads) {
-        const int w = e / (2 * share), f = e / share % 2, rr = r0 + e % share;
-        all[e] = ld_cluster(mapa_shared(stat + (rr / BM) * 2 * BM + f * BM + rr % BM, w));
-      }
-      __syncthreads();
-      for (int e = threadIdx.x; e < share * (DH / 8); e += kThreads) {
-        const int rr = r0 + e % share, oct = e / share;
-        const int sl = rr / BM, row = rr % BM, tok = row / p.group, i = it.i0 + sl * p.tq + tok;
-        if (tok >= p.tq || i >= it.n) continue;
-        int row_lo, row_hi;
-        visible(it.kv - it.n + i, it.kv, p.a.dlo, p.a.dhi, row_lo, row_hi);
-        const float* st = all + rr - r0;
-        float M = -INFINITY, sum = 0.0f;
-        for (int w = 0; w < ranks; ++w) M = max2n(M, st[w * 2 * share]);
-        float acc[8] = {};
-        for (int w = 0; w < ranks; ++w) {
-          const float lw = st[(w * 2 + 1) * share];
-          if (lw == 0.0f) continue;  // no visible key in this run (a NaN sum is taken)
-          const float a = ex2(st[w * 2 * share] - M);
-          sum = fmaf(a, lw, sum);
-          const uint32_t src = mapa_shared(smem + sl * L::PART + (2 * oct * BM + row) * 16, w);
-          const float4 u = ld_cluster4(src), v = ld_cluster4(src + BM * 16);
-          acc[0] = fmaf(a, u.x, acc[0]); acc[1] = fmaf(a, u.y, acc[1]);
-          acc[2] = fmaf(a, u.z, acc[2]); acc[3] = fmaf(a, u.w, acc[3]);
-          acc[4] = fmaf(a, v.x, acc[4]); acc[5] = fmaf(a, v.y, acc[5]);
-          acc[6] = fmaf(a, v.z, acc[6]); acc[7] = fmaf(a, v.w, acc[7]);
-        }
-        const bool empty = row_lo > row_hi;
-        const float inv = 1.0f / sum;
-        float check = 0.0f;
-        uint32_t w4[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          check = fmaf(acc[2 * q] * inv, 0.0f, fmaf(acc[2 * q + 1] * inv, 0.0f, check));
-          w4[q] = empty ? 0u : pack2<BF16>(acc[2 * q] * inv, acc[2 * q + 1] * inv);
-        }
-        if (!empty && !(check == 0.0f)) {
-          atomicOr(&redo[rr >> 5], 1u << (rr & 31));
-        } else {
-          uint16_t* out = p.a.out + static_cast<int64_t>(it.q0 + i) * p.a.ldo +
-                          (it.g * p.group + row - tok * p.group) * DH + oct * 8;
-          *reinterpret_cast<uint4*>(out) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
-        }
-      }
-      __syncthreads();
-      for (int rr = r0 + warp; rr < r0 + share; rr += kThreads / 32)
-        if (redo[rr >> 5] >> (rr & 31) & 1) {
-          const int row = rr % BM, tok = row / p.group;
+    if (SPLIT) __syncthreads();
+    if (!SPLIT && redo[0] && !*abort_flag) {  // (redo is read after the barrier above)
+      // The marked rows of this CTA's units, again from the definition.
+      Finder finder;
+      finder.init(p);
+      for (int k = 0;; ++k) {
+        const Item it = make_item(p, finder, unit_of(k), 0, 1);
+        if (it.b < 0) break;
+        for (int rr = warp - kSoftWarp0; rr < 2 * p.tq * p.group; rr += kSoftThreads / 32) {
+          const int i = it.i0 + rr / p.group, head = it.g * p.group + rr % p.group;
+          if (i >= it.n) break;
+          const uint16_t mark = p.a.out[static_cast<int64_t>(it.q0 + i) * p.a.ldo + head * DH];
+          if ((mark & 0x7fffu) != 0x7fffu) continue;
           const Seq seq{it.q0, it.n, it.kv};
-          const int i = it.i0 + (rr / BM) * p.tq + tok, head = it.g * p.group + row - tok * p.group;
           if (p.a.kv.table) row_attention<DH, BF16, true>(p.a, it.b, seq, i, head);
           else row_attention<DH, BF16, false>(p.a, it.b, seq, i, head);
         }
+      }
     }
-    cluster_sync_all();  // no CTA leaves while its partials are read
+    if (SPLIT) {
+      cluster_sync_all();  // every partial is written
+      const Item it = items[0];
+      if (it.b >= 0 && !*abort_flag) {
+        const float* stat = reinterpret_cast<const float*>(smem + 2 * L::PART);       // [slot][m, l][BM]
+        float* all = reinterpret_cast<float*>(smem + 2 * L::PART) + 4 * BM;           // [rank][slot][m, l][rows]
+        // Rank k finishes the rows [k, k + 1) * 2 BM / ranks.
+        const int share = 2 * BM / ranks, r0 = rank * share;
+        for (int e = threadIdx.x - kSoftWarp0 * 32; e < ranks * 2 * share; e += kSoftThreads) {
+          const int w = e / (2 * share), f = e / share % 2, rr = r0 + e % share;
+          all[e] = ld_cluster(mapa_shared(stat + (rr / BM) * 2 * BM + f * BM + rr % BM, w));
+        }
+        soft_sync();
+        for (int e = threadIdx.x - kSoftWarp0 * 32; e < share * (DH / 8); e += kSoftThreads) {
+          const int rr = r0 + e % share, oct = e / share;
+          const int sl = rr / BM, row = rr % BM, tok = row / p.group, i = it.i0 + sl * p.tq + tok;
+          if (tok >= p.tq || i >= it.n) continue;
+          int row_lo, row_hi;
+          visible(it.kv - it.n + i, it.kv, p.a.dlo, p.a.dhi, row_lo, row_hi);
+          const float* st = all + rr - r0;
+          float M = -INFINITY, sum = 0.0f;
+          for (int w = 0; w < ranks; ++w) M = max2n(M, st[w * 2 * share]);
+          float acc[8] = {};
+          for (int w = 0; w < ranks; ++w) {
+            const float lw = st[(w * 2 + 1) * share];
+            if (lw == 0.0f) continue;  // no visible key in this run (a NaN sum is taken)
+            const float a = ex2(st[w * 2 * share] - M);
+            sum = fmaf(a, lw, sum);
+            const uint32_t src = mapa_shared(smem + sl * L::PART + (2 * oct * BM + row) * 16, w);
+            const float4 u = ld_cluster4(src), v = ld_cluster4(src + BM * 16);
+            acc[0] = fmaf(a, u.x, acc[0]); acc[1] = fmaf(a, u.y, acc[1]);
+            acc[2] = fmaf(a, u.z, acc[2]); acc[3] = fmaf(a, u.w, acc[3]);
+            acc[4] = fmaf(a, v.x, acc[4]); acc[5] = fmaf(a, v.y, acc[5]);
+            acc[6] = fmaf(a, v.z, acc[6]); acc[7] = fmaf(a, v.w, acc[7]);
+          }
+          const bool empty = row_lo > row_hi;
+          const float inv = 1.0f / sum;
+          float check = 0.0f;
+          uint32_t w4[4];
+  #pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            check = fmaf(acc[2 * q] * inv, 0.0f, fmaf(acc[2 * q + 1] * inv, 0.0f, check));
+            w4[q] = empty ? 0u : pack2<BF16>(acc[2 * q] * inv, acc[2 * q + 1] * inv);
+          }
+          if (!empty && !(check == 0.0f)) {
+            atomicOr(&redo[rr >> 5], 1u << (rr & 31));
+          } else {
+            uint16_t* out = p.a.out + static_cast<int64_t>(it.q0 + i) * p.a.ldo +
+                            (it.g * p.group + row - tok * p.group) * DH + oct * 8;
+            *reinterpret_cast<uint4*>(out) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
+          }
+        }
+        soft_sync();
+        for (int rr = r0 + warp - kSoftWarp0; rr < r0 + share; rr += kSoftThreads / 32)
+          if (redo[rr >> 5] >> (rr & 31) & 1) {
+            const int row = rr % BM, tok = row / p.group;
+            const Seq seq{it.q0, it.n, it.kv};
+            const int i = it.i0 + (rr / BM) * p.tq + tok, head = it.g * p.group + row - tok * p.group;
+            if (p.a.kv.table) row_attention<DH, BF16, true>(p.a, it.b, seq, i, head);
+            else row_attention<DH, BF16, false>(p.a, it.b, seq, i, head);
+          }
+      }
+      cluster_sync_all();  // no CTA leaves while its partials are read
+    }
   }
 }
 
@@ -926,8 +934,12 @@ int launch_tile(const CUtensorMap* tm, const TileParams& p, unsigned grid, int r
   cudaGetDevice(&dev);
   const uint64_t bit = 1ull << (dev & 63);
   if (!(configured.load() & bit)) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::BYTES) != cudaSuccess)
+    cudaFuncAttributes fa;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::BYTES) != cudaSuccess ||
+        cudaFuncGetAttributes(&fa, kernel) != cudaSuccess)
       return report_error(RB_E_DEVICE, "ragged attention: kernel attributes");
+    // A warpgroup that asks for more than the launch holds would wait forever.
+    if (fa.numRegs != kLaunchRegs) return report_error(RB_E_DEVICE, "ragged attention: register split");
     configured |= bit;
   }
   cudaLaunchConfig_t cfg{};
