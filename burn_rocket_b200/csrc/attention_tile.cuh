@@ -318,12 +318,12 @@ tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
   uint64_t* o_free = o_done + 2;       // [slot] the unit's O was read out
   uint64_t* i_full = o_free + 2;       // [2] an item is there
   uint64_t* i_empty = i_full + 2;      // [2] every role has read it
-  uint64_t* turns = i_empty + 2;       // [lane quarter][slot] whose exponentials run
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(turns + 8);
+  uint64_t* p_half = i_empty + 2;      // [slot] the first half of P is in TMEM
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(p_half + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   uint32_t* redo = tmem_slot + 2;      // [8] rows to compute again (one a bit when split, else a flag)
   Item* items = reinterpret_cast<Item*>(redo + 8);  // [2]
-  static_assert((2 + 2 * KS + 2 * VS + 20) * 8 + 48 + 2 * sizeof(Item) <= 1024, "barrier area");
+  static_assert((2 + 2 * KS + 2 * VS + 14) * 8 + 48 + 2 * sizeof(Item) <= 1024, "barrier area");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t* err = p.a.seqs.err;
@@ -337,12 +337,12 @@ tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
+      mbar_init(&p_half[i], 4);
       mbar_init(&o_done[i], 1);
       mbar_init(&o_free[i], 4);
       mbar_init(&i_full[i], 1);
       mbar_init(&i_empty[i], 9);
     }
-    for (int i = 0; i < 8; ++i) mbar_init(&turns[i], 1);
     *abort_flag = 0;
     for (int i = 0; i < 8; ++i) redo[i] = 0;
     fence_mbar_init();
@@ -529,7 +529,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
           bool v_ready = false;
           for (int s = 0; ok && s < 2; ++s) {
             if (!(rlo[s] <= j && j <= rhi[s])) continue;
-            if (!(ok = mbar_wait(&p_full[s], n_pv[s] & 1, err, abort_flag))) break;
+            if (!(ok = mbar_wait(&p_half[s], n_pv[s] & 1, err, abort_flag))) break;
             tc_fence_after();
             if (first_pv[s] && n_out[s] > 0) {  // the last unit's O must be out
               if (!(ok = mbar_wait(&o_free[s], (n_out[s] - 1) & 1, err, abort_flag))) break;
@@ -541,14 +541,19 @@ tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
               v_ready = true;
             }
             const uint32_t o_tmem = tmem_base + s * 256 + 128, p_tmem = tmem_base + s * 256;
-#pragma unroll
-            for (int ks = 0; ks < BN / 16; ++ks) {
+            auto pv = [&](int ks) {
               const uint32_t acc = (!first_pv[s] || ks > 0) ? 1u : 0u;
               umma_f16_ts(o_tmem, p_tmem + ks * 8, desc_add(v_desc, vs * L::KV_TILE + ks * 2048), idesc_o, acc);
               if (L::TAIL)
                 umma_f16_ts(o_tmem + L::ATOMS * 64, p_tmem + ks * 8,
                             desc_add(vt_desc, vs * L::KV_TILE + L::KV_TAIL_OFF + ks * 512), idesc_ot, acc);
-            }
+            };
+#pragma unroll
+            for (int ks = 0; ks < BN / 32; ++ks) pv(ks);
+            if (!(ok = mbar_wait(&p_full[s], n_pv[s] & 1, err, abort_flag))) break;
+            tc_fence_after();
+#pragma unroll
+            for (int ks = BN / 32; ks < BN / 16; ++ks) pv(ks);
             umma_commit(&o_done[s]);
             ++n_pv[s];
             first_pv[s] = false;
@@ -589,17 +594,6 @@ tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
     const uint32_t s_col = s * 256, o_col = s * 256 + 128;
     const int tok = row / p.group, sub = row - tok * p.group;
     int it_n = 0, kv_base = 0;
-    // The warp of the other slot on the same lanes sits on the same
-    // sub-partition: they take turns, tile by tile, at the exponentials, slot 0
-    // first. Left alone both slots run them together at half the MUFU's rate
-    // each and then wait for the tensor pipe together.
-    uint64_t* my_turn = &turns[(warp & 3) * 2 + s];
-    uint64_t* its_turn = &turns[(warp & 3) * 2 + (s ^ 1)];
-    int n_turn = 0;
-    if (s == 1 && lane == 0) mbar_arrive(its_turn);
-    auto take_turn = [&]() -> bool {
-      return __all_sync(0xffffffffu, mbar_wait(my_turn, n_turn++ & 1, err, abort_flag));
-    };
     Item it;
     for (int k = 0;; ++k) {
       if (!__all_sync(0xffffffffu, get_item(k, it))) break;
@@ -617,13 +611,8 @@ tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
       visible(first_pos + min(it.n, ia + p.tq) - 1, it.kv, p.a.dlo, p.a.dhi, all_lo, x0);
       float m_used = -INFINITY, l = 0.0f;
       bool ok = true;
-      for (int j = it.ja; ok && j <= it.jb; ++j) {
-        if (j < lo || j > hi) {  // the other slot's tile: pass the turn on
-          ok = take_turn();
-          if (lane == 0) mbar_arrive(its_turn);
-          continue;
-        }
-        if (!__all_sync(0xffffffffu, mbar_wait(&s_full[s], it_n++ & 1, err, abort_flag))) {
+      for (int j = lo; j <= hi; ++j, ++it_n) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&s_full[s], it_n & 1, err, abort_flag))) {
           ok = false;
           break;
         }
@@ -681,7 +670,9 @@ tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
           need = true;
         }
         const float nm = m_used == -INFINITY ? 0.0f : -m_used;  // nothing visible yet: weights are 0
-        if (!(ok = take_turn())) break;
+        // The first 64 keys' weights go to P·V while the others are computed,
+        // unless O or V has to be touched first.
+        const bool late = __any_sync(0xffffffffu, need) || it.kv - ka < BN;
         uint64_t rs[2] = {0ull, 0ull};
 #pragma unroll
         for (int c0 = 0; c0 < BN; c0 += 32) {
@@ -695,9 +686,14 @@ tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
             rs[(e / 2) & 1] = f2_add(rs[(e / 2) & 1], f2_pack(p0, p1));
             pk[e / 2] = pack2<BF16>(p0, p1);
           }
+          if (c0 == 64 && !late) {  // (here, where the first half's stores are long done)
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_half[s]);
+          }
           tmem_st16(lane_base + s_col + c0 / 2, pk);
         }
-        if (lane == 0) mbar_arrive(its_turn);
         float a0, a1, a2, a3;
         f2_unpack(rs[0], a0, a1);
         f2_unpack(rs[1], a2, a3);
@@ -743,7 +739,10 @@ tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[s]);
+        if (lane == 0) {
+          if (late) mbar_arrive(&p_half[s]);
+          mbar_arrive(&p_full[s]);
+        }
       }
       if (!ok) break;
       kv_base += max(0, it.jb - it.ja + 1);
