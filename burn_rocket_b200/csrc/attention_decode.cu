@@ -109,10 +109,44 @@ __device__ __forceinline__ float ld_cluster(uint32_t addr) {
   return v;
 }
 
+// The sequence with r longer ones before it (of equal ones the lower index
+// first), among at most 128: bisection on the key count, four sequences a lane.
+__device__ __forceinline__ int ranked_sequence(const RaggedBatch& q, int r) {
+  const int lane = threadIdx.x & 31;
+  int kv[4], hi = 0;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const int b = 32 * g + lane;
+    kv[g] = b < q.batch ? max(0, min(__ldg(q.kv_len + b), q.max_kv)) : -1;
+    hi = max(hi, kv[g]);
+  }
+  auto above = [&](int x) {  // sequences with more than x keys
+    return __reduce_add_sync(0xffffffffu, (kv[0] > x) + (kv[1] > x) + (kv[2] > x) + (kv[3] > x));
+  };
+  int lo = -1;  // above(lo) > r >= above(hi)
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (above(mid) > r) lo = mid;
+    else hi = mid;
+  }
+  int idx = r - above(hi), b = 0;  // among those with exactly hi keys
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const unsigned m = __ballot_sync(0xffffffffu, kv[g] == hi);
+    const int c = __popc(m);
+    if (idx >= 0 && idx < c) b = 32 * g + __fns(m, 0, idx + 1);
+    idx -= c;
+  }
+  return b;
+}
+
 // Grid: ((sequence * row tiles + row tile) * KV heads + KV head) * cluster
 // size + rank; neighbouring clusters read neighbouring heads of the same slots.
+// Where the grid is more than the GPU holds at a time, `longest_first` sends the
+// long sequences ahead.
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kWarps * 32, 2) decode_kernel(const __grid_constant__ AttnRagged p, int row_tiles) {
+__global__ void __launch_bounds__(kWarps * 32, 2) decode_kernel(const __grid_constant__ AttnRagged p, int row_tiles, bool longest_first) {
   using G = Geo<D>;
   extern __shared__ __align__(128) uint8_t smem[];
   const uint32_t ranks = cluster_size(), rank = cluster_ctarank();
@@ -120,7 +154,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) decode_kernel(const __grid_con
   const int unit = blockIdx.x / ranks;
   const int head_kv = unit % p.n_kv_heads;
   const int tile = unit / p.n_kv_heads % row_tiles;
-  const int b = unit / p.n_kv_heads / row_tiles;
+  int b = unit / p.n_kv_heads / row_tiles;
+  if (longest_first) b = ranked_sequence(p.seqs, b);
   const int group = p.n_head / p.n_kv_heads;
   const Seq s = load_seq(p.seqs, b);
   const int row0 = tile * kRows, rows = min(kRows, s.n * group - row0);
@@ -315,8 +350,9 @@ __global__ void __launch_bounds__(kWarps * 32, 2) decode_kernel(const __grid_con
     if (e % kRows < rows)
       all[e] = ld_cluster(mapa_shared(stat + kWarps * 2 * kRows + e % (2 * kRows), e / (2 * kRows)));
   __syncthreads();
-  // Each rank finishes its share of the columns.
-  const int cols = D / ranks, c0 = rank * cols;
+  // Each rank finishes its share of the columns, in groups of four.
+  const int c0 = static_cast<int>(rank * (D / 4) / ranks) * 4, c1 = static_cast<int>((rank + 1) * (D / 4) / ranks) * 4;
+  const int cols = c1 - c0;
   for (int e = threadIdx.x; e < rows * cols; e += kWarps * 32) {
     const int r = e / cols, col = c0 + e % cols;
     float M = -INFINITY, acc = 0.0f, sum = 0.0f;
@@ -339,36 +375,74 @@ __global__ void __launch_bounds__(kWarps * 32, 2) decode_kernel(const __grid_con
   const int again = *redo;
   for (int r = warp; r < rows; r += kWarps)
     if (again >> r & 1)
-      row_attention<D, BF16, true>(p, b, s, (row0 + r) / group, head_kv * group + (row0 + r) % group, c0, c0 + cols);
+      row_attention<D, BF16, true>(p, b, s, (row0 + r) / group, head_kv * group + (row0 + r) % group, c0, c1);
+}
+
+// Cluster size for one call. Measured on this kernel (flushed L2): a CTA alone
+// streams a 128-wide key (512 bytes) in 14 ns, the GPU 6.3 TB/s, and each wave of
+// clusters costs 5 us more. 8 x 4096 keys x 8 heads: sizes 1, 2, 4, 8 took 63,
+// 41, 37, 43 us; 64 x 4096: 184, 197, 209, 238; 3 x 33000 sizes 8, 10, 12, 16:
+// 84, 80, 92, 96 (sizes above 10 leave fewer than 24 clusters resident); 64
+// sequences of 33 to 8100 keys x 4 heads 1, 2, 3, 4, 8: 147, 109, 119, 125, 158.
+static int pick_ranks(const int* active, int64_t units, int batch, double keys, int d) {
+  const double key_ns = 14.0 * d / 128;
+  const double all_ns = 0.6 * units * keys * d * 4 / 6300.0 * active[1];  // (lengths vary: most lie below the longest)
+  int best = 1;
+  double least = 1e30;
+  for (int r = 1; r <= 16; ++r) {
+    if (active[r] <= 0 || (r > 1 && keys < r * kWarps * kRows)) continue;
+    const double waves = static_cast<double>((units + active[r] - 1) / active[r]), run = keys / r * key_ns;
+    const double all = all_ns / (active[r] * r);  // sizes that leave SMs empty stream less
+    // A few sequences are alike: each wave lasts as long. Many even out, but
+    // for the last long ones.
+    const double cost = batch <= 4 ? std::max(all, waves * run) + 5000.0 * waves
+                                   : std::max(all, run) + 0.35 * run + 5000.0 * waves;
+    if (cost < least) least = cost, best = r;
+  }
+  return best;
 }
 
 template <int D, bool BF16>
-static int launch(const AttnRagged& a, int ranks, int row_tiles, cudaStream_t st) {
-  static std::atomic<uint64_t> configured{0};
+static int launch(const AttnRagged& a, int row_tiles, cudaStream_t st) {
+  auto kernel = decode_kernel<D, BF16>;
+  static std::atomic<int> resident[64][17];  // clusters of each size that a device holds; [0]: known
   int dev = 0;
   cudaGetDevice(&dev);
-  const uint64_t bit = 1ull << (dev & 63);
-  if (!(configured.load() & bit)) {
-    if (cudaFuncSetAttribute(decode_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo<D>::BYTES) !=
-            cudaSuccess ||
-        cudaFuncSetAttribute(decode_kernel<D, BF16>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
-      return report_error(RB_E_DEVICE, "attention_paged: kernel attributes");
-    configured |= bit;
-  }
-  const int64_t blocks = static_cast<int64_t>(a.seqs.batch) * row_tiles * a.n_kv_heads * ranks;
-  if (blocks > 0x7fffffff) return report_error(RB_E_SHAPE, "attention_paged: batch too large");
+  if (dev < 0 || dev >= 64) return report_error(RB_E_DEVICE, "attention_paged: device ordinal");
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
   cfg.blockDim = dim3(kWarps * 32);
   cfg.dynamicSmemBytes = Geo<D>::BYTES;
-  cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = ranks;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[0].val.clusterDim.x = at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
+  cfg.numAttrs = 1;
+  if (!resident[dev][0].load(std::memory_order_acquire)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Geo<D>::BYTES) != cudaSuccess ||
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+      return report_error(RB_E_DEVICE, "attention_paged: kernel attributes");
+    for (int r = 1; r <= 16; ++r) {
+      int n = 0;
+      at[0].val.clusterDim.x = r;
+      cfg.gridDim = dim3(r);
+      if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) n = 0;
+      resident[dev][r] = n;
+    }
+    cudaGetLastError();
+    resident[dev][0].store(1, std::memory_order_release);
+  }
+  int active[17];
+  for (int r = 1; r <= 16; ++r) active[r] = resident[dev][r].load(std::memory_order_relaxed);
+  const int64_t units = static_cast<int64_t>(a.seqs.batch) * a.n_kv_heads * row_tiles;
+  const int keys = a.dlo <= -kRaggedNoBound ? a.hint_kv : std::min(a.hint_kv, a.seqs.max_q - a.dlo);
+  const int ranks = pick_ranks(active, units, a.seqs.batch, std::max(keys, 1), D);
+  if (units * ranks > 0x7fffffff) return report_error(RB_E_SHAPE, "attention_paged: batch too large");
+  const bool longest_first = units > active[ranks] && a.seqs.batch > 1 && a.seqs.batch <= 128;
+  cfg.gridDim = dim3(static_cast<unsigned>(units * ranks));
+  cfg.stream = st;
+  at[0].val.clusterDim.x = ranks;
   cfg.numAttrs = ranks > 1 ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, decode_kernel<D, BF16>, a, row_tiles);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, row_tiles, longest_first);
   return e == cudaSuccess ? RB_OK : report_error(RB_E_DEVICE, cudaGetErrorString(e));
 }
 
@@ -378,13 +452,8 @@ int launch_attention_decode(const AttnRagged& a, cudaStream_t st) {
   using namespace decode;
   const int group = a.n_head / a.n_kv_heads;
   const int row_tiles = static_cast<int>((static_cast<int64_t>(a.seqs.max_q) * group + kRows - 1) / kRows);
-  const int64_t units = static_cast<int64_t>(a.seqs.batch) * a.n_kv_heads * row_tiles;
-  int ranks = 1;
-  const int keys = a.dlo <= -kRaggedNoBound ? a.hint_kv : std::min(a.hint_kv, a.seqs.max_q - a.dlo);
-  while (ranks < 16 && units * ranks < 4ll * a.num_sms && keys > ranks * kWarps * kRows) ranks *= 2;
-  if (a.head_dim == 128)
-    return a.bf16 ? launch<128, true>(a, ranks, row_tiles, st) : launch<128, false>(a, ranks, row_tiles, st);
-  return a.bf16 ? launch<64, true>(a, ranks, row_tiles, st) : launch<64, false>(a, ranks, row_tiles, st);
+  if (a.head_dim == 128) return a.bf16 ? launch<128, true>(a, row_tiles, st) : launch<128, false>(a, row_tiles, st);
+  return a.bf16 ? launch<64, true>(a, row_tiles, st) : launch<64, false>(a, row_tiles, st);
 }
 
 }  // namespace rb

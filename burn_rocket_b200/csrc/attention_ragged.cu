@@ -48,13 +48,11 @@ static int launch_attention_tile(const AttnRagged& a, cudaStream_t st) {
   // At most this many units: every sequence ends in one part-filled span.
   const int64_t units = (static_cast<int64_t>(a.seqs.tokens) / span + std::min(a.seqs.batch, a.seqs.tokens)) * a.n_kv_heads;
   if (units > 0x7fffffff) return report_error(RB_E_SHAPE, "ragged attention: batch too large");
-  // Fewer units than half the SMs: a cluster a unit, two key tiles a CTA at least.
-  int ranks = 1;
+  // The keys of the longest unit: a window's, or the expected length.
   const int keys = a.dlo <= -kRaggedNoBound ? a.hint_kv : std::min(a.hint_kv, span - 1 - a.dlo + std::max(a.dhi, 0));
-  while (ranks < 8 && units * ranks * 2 <= a.num_sms && keys >= ranks * 4 * BN) ranks *= 2;
-  const unsigned grid = static_cast<unsigned>(ranks > 1 ? units * ranks : std::min<int64_t>(units, a.num_sms));
-  if (d == 128) return launch_d128(tm, p, grid, ranks, st);
-  return d == 64 ? launch_d64(tm, p, grid, ranks, st) : launch_d80(tm, p, grid, ranks, st);
+  const Work w{units, (keys + BN - 1) / BN};
+  if (d == 128) return launch_d128(tm, p, w, st);
+  return d == 64 ? launch_d64(tm, p, w, st) : launch_d80(tm, p, w, st);
 }
 
 int launch_attention_ragged(const AttnRagged& a, cudaStream_t st) {

@@ -865,7 +865,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
         const float* stat = reinterpret_cast<const float*>(smem + 2 * L::PART);       // [slot][m, l][BM]
         float* all = reinterpret_cast<float*>(smem + 2 * L::PART) + 4 * BM;           // [rank][slot][m, l][rows]
         // Rank k finishes the rows [k, k + 1) * 2 BM / ranks.
-        const int share = 2 * BM / ranks, r0 = rank * share;
+        const int r0 = rank * 2 * BM / ranks, share = (rank + 1) * 2 * BM / ranks - r0;
         for (int e = threadIdx.x - kSoftWarp0 * 32; e < ranks * 2 * share; e += kSoftThreads) {
           const int w = e / (2 * share), f = e / share % 2, rr = r0 + e % share;
           all[e] = ld_cluster(mapa_shared(stat + (rr / BM) * 2 * BM + f * BM + rr % BM, w));
@@ -925,22 +925,14 @@ tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
   }
 }
 
+// How many units a call has at most, and how many key tiles the longest.
+struct Work {
+  int64_t units;
+  int tiles;
+};
+
 template <int D, bool BF16, bool SOFTCAP, bool SPLIT>
-int launch_tile(const CUtensorMap* tm, const TileParams& p, unsigned grid, int ranks, cudaStream_t st) {
-  auto kernel = tile_kernel<D, BF16, SOFTCAP, SPLIT>;
-  static std::atomic<uint64_t> configured{0};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  const uint64_t bit = 1ull << (dev & 63);
-  if (!(configured.load() & bit)) {
-    cudaFuncAttributes fa;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::BYTES) != cudaSuccess ||
-        cudaFuncGetAttributes(&fa, kernel) != cudaSuccess)
-      return report_error(RB_E_DEVICE, "ragged attention: kernel attributes");
-    // A warpgroup that asks for more than the launch holds would wait forever.
-    if (fa.numRegs != kLaunchRegs) return report_error(RB_E_DEVICE, "ragged attention: register split");
-    configured |= bit;
-  }
+int launch_kernel(const CUtensorMap* tm, const TileParams& p, unsigned grid, int ranks, cudaStream_t st) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(kThreads);
@@ -952,23 +944,72 @@ int launch_tile(const CUtensorMap* tm, const TileParams& p, unsigned grid, int r
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = SPLIT ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, tm[0], tm[1], tm[2], tm[3], tm[4], tm[5], p);
+  const cudaError_t e =
+      cudaLaunchKernelEx(&cfg, tile_kernel<D, BF16, SOFTCAP, SPLIT>, tm[0], tm[1], tm[2], tm[3], tm[4], tm[5], p);
   return e == cudaSuccess ? RB_OK : report_error(RB_E_DEVICE, cudaGetErrorString(e));
 }
 
-template <int D, bool SPLIT>
-int launch_types(const CUtensorMap* tm, const TileParams& p, unsigned grid, int ranks, cudaStream_t st) {
+// Per device and kernel pair: attributes set, the register split checked, and
+// the clusters of each size that the device holds.
+template <int D, bool BF16, bool SOFTCAP>
+int launch_tile(const CUtensorMap* tm, const TileParams& p, const Work& w, cudaStream_t st) {
+  static std::atomic<int> resident[64][9];  // [0]: known
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return report_error(RB_E_DEVICE, "ragged attention: device ordinal");
+  if (!resident[dev][0].load(std::memory_order_acquire)) {
+    auto whole = tile_kernel<D, BF16, SOFTCAP, false>;
+    auto split = tile_kernel<D, BF16, SOFTCAP, true>;
+    cudaFuncAttributes fw, fs;
+    if (cudaFuncSetAttribute(whole, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::BYTES) != cudaSuccess ||
+        cudaFuncSetAttribute(split, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::BYTES) != cudaSuccess ||
+        cudaFuncGetAttributes(&fw, whole) != cudaSuccess || cudaFuncGetAttributes(&fs, split) != cudaSuccess)
+      return report_error(RB_E_DEVICE, "ragged attention: kernel attributes");
+    // A warpgroup that asks for more than the launch holds would wait forever.
+    if (fw.numRegs != kLaunchRegs || fs.numRegs != kLaunchRegs)
+      return report_error(RB_E_DEVICE, "ragged attention: register split");
+    for (int r = 1; r <= 8; ++r) {
+      cudaLaunchConfig_t cfg{};
+      cfg.gridDim = dim3(r);
+      cfg.blockDim = dim3(kThreads);
+      cfg.dynamicSmemBytes = Smem<D>::BYTES;
+      cudaLaunchAttribute at[1];
+      at[0].id = cudaLaunchAttributeClusterDimension;
+      at[0].val.clusterDim.x = r;
+      at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+      cfg.attrs = at;
+      cfg.numAttrs = 1;
+      int n = 0;
+      if (cudaOccupancyMaxActiveClusters(&n, split, &cfg) != cudaSuccess) n = 0;
+      resident[dev][r] = n;
+    }
+    cudaGetLastError();
+    resident[dev][0].store(1, std::memory_order_release);
+  }
+  // A cluster a unit only while every unit finds one at once, and two key tiles
+  // a CTA at least: a second wave costs more than the split gains (2 x 8000 keys,
+  // 16 new tokens, 8 KV heads: 65 us with 16 clusters of 8, of which 14 are
+  // resident).
+  int ranks = 1;
+  for (int r = 2; r <= 8; ++r)
+    if (w.units <= resident[dev][r].load(std::memory_order_relaxed) && w.tiles >= 2 * r) ranks = r;
+  if (ranks > 1)
+    return launch_kernel<D, BF16, SOFTCAP, true>(tm, p, static_cast<unsigned>(w.units * ranks), ranks, st);
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(w.units, p.a.num_sms));
+  return launch_kernel<D, BF16, SOFTCAP, false>(tm, p, grid, 1, st);
+}
+
+template <int D>
+int launch_types(const CUtensorMap* tm, const TileParams& p, const Work& w, cudaStream_t st) {
   if (p.a.softcap != 0.0f)
-    return p.a.bf16 ? launch_tile<D, true, true, SPLIT>(tm, p, grid, ranks, st)
-                    : launch_tile<D, false, true, SPLIT>(tm, p, grid, ranks, st);
-  return p.a.bf16 ? launch_tile<D, true, false, SPLIT>(tm, p, grid, ranks, st)
-                  : launch_tile<D, false, false, SPLIT>(tm, p, grid, ranks, st);
+    return p.a.bf16 ? launch_tile<D, true, true>(tm, p, w, st) : launch_tile<D, false, true>(tm, p, w, st);
+  return p.a.bf16 ? launch_tile<D, true, false>(tm, p, w, st) : launch_tile<D, false, false>(tm, p, w, st);
 }
 
 // Instantiated one head width a file, so that they compile side by side.
-int launch_d64(const CUtensorMap* tm, const TileParams& p, unsigned grid, int ranks, cudaStream_t st);
-int launch_d80(const CUtensorMap* tm, const TileParams& p, unsigned grid, int ranks, cudaStream_t st);
-int launch_d128(const CUtensorMap* tm, const TileParams& p, unsigned grid, int ranks, cudaStream_t st);
+int launch_d64(const CUtensorMap* tm, const TileParams& p, const Work& w, cudaStream_t st);
+int launch_d80(const CUtensorMap* tm, const TileParams& p, const Work& w, cudaStream_t st);
+int launch_d128(const CUtensorMap* tm, const TileParams& p, const Work& w, cudaStream_t st);
 
 }  // namespace tile
 

@@ -3,8 +3,8 @@
 
 namespace rb {
 namespace tile {
-int launch_d128(const CUtensorMap* tm, const TileParams& p, unsigned grid, int ranks, cudaStream_t st) {
-  return ranks > 1 ? launch_types<128, true>(tm, p, grid, ranks, st) : launch_types<128, false>(tm, p, grid, 1, st);
+int launch_d128(const CUtensorMap* tm, const TileParams& p, const Work& w, cudaStream_t st) {
+  return launch_types<128>(tm, p, w, st);
 }
 }  // namespace tile
 }  // namespace rb

@@ -4,8 +4,8 @@
 
 namespace rb {
 namespace tile {
-int launch_d80(const CUtensorMap* tm, const TileParams& p, unsigned grid, int ranks, cudaStream_t st) {
-  return ranks > 1 ? launch_types<80, true>(tm, p, grid, ranks, st) : launch_types<80, false>(tm, p, grid, 1, st);
+int launch_d80(const CUtensorMap* tm, const TileParams& p, const Work& w, cudaStream_t st) {
+  return launch_types<80>(tm, p, w, st);
 }
 }  // namespace tile
 }  // namespace rb
