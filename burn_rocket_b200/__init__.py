@@ -360,11 +360,11 @@ def _refuse(op: str, detail: str, m: int = 0):
     raise OpFailure(Error(op, _lib.RB_E_SHAPE), m, detail=detail)
 
 
-def _on(op: str, dev: int, dtype, **tensors) -> None:
+def _on(op: str, dev: int, dtype, *tensors) -> None:
     """Every tensor on CUDA device `dev` and of the given dtype."""
-    for what, t in tensors.items():
-        if t.dtype is not dtype or t.get_device() != dev or not t.is_cuda:
-            _refuse(op, f"{what} must be {dtype} on cuda:{dev}, got {t.dtype} on {t.device}")
+    for t in tensors:
+        if t.dtype is not dtype or t.get_device() != dev:
+            _refuse(op, f"expected {dtype} tensors on cuda:{dev}, got {t.dtype} on {t.device}")
 
 
 def _rows(op: str, what: str, t, tokens: int, width: int) -> int:
@@ -378,28 +378,24 @@ def _rows(op: str, what: str, t, tokens: int, width: int) -> int:
 
 
 def _device_of(op: str, q) -> int:
-    if not q.is_cuda or q.dim() != 2:
+    dev = q.get_device()  # -1: not a CUDA tensor
+    if dev < 0 or q.dim() != 2:
         _refuse(op, "expected 2-D CUDA tensors")
-    dev = q.get_device()
-    if _device is not None and dev != _device:
+    if dev != _device and _device is not None:
         _refuse(op, f"tensors on cuda:{dev}, the engine is on cuda:{_device}")
     return dev
 
 
-def _bounds(op: str, dev: int, cu) -> int:
-    """Batch size of sequence bounds int32 [batch + 1]."""
-    import torch
-    _on(op, dev, torch.int32, cu=cu)
-    if cu.dim() != 1 or cu.shape[0] < 1 or not cu.is_contiguous():
-        _refuse(op, f"cu must be a contiguous int32 [batch + 1], got {tuple(cu.shape)}")
-    return cu.shape[0] - 1
+def _bounds(op: str, cu) -> int:
+    """Batch size of sequence bounds [batch + 1]."""
+    batch = cu.numel() - 1
+    if batch < 0 or cu.dim() != 1 or not cu.is_contiguous():
+        _refuse(op, f"the sequence bounds must be a contiguous int32 [batch + 1], got {tuple(cu.shape)}")
+    return batch
 
 
-def _cache(op: str, dev: int, dtype, k_cache, v_cache, page_table, kv_len, batch: int, n_kv_heads: int, head_dim: int):
+def _cache(op: str, k_cache, v_cache, page_table, kv_len, batch: int, n_kv_heads: int, head_dim: int):
     """(page stride, pages, page size, table width) of a paged cache."""
-    import torch
-    _on(op, dev, dtype, k_cache=k_cache, v_cache=v_cache)
-    _on(op, dev, torch.int32, page_table=page_table, kv_len=kv_len)
     shape, strides = k_cache.shape, k_cache.stride()
     row = n_kv_heads * head_dim
     ok = len(shape) == 4 and shape[2] == n_kv_heads and shape[3] == head_dim and v_cache.shape == shape
@@ -410,19 +406,28 @@ def _cache(op: str, dev: int, dtype, k_cache, v_cache, page_table, kv_len, batch
     if not ok:
         _refuse(op, f"k_cache and v_cache must be alike, [pages, page_size, {n_kv_heads}, {head_dim}] with contiguous "
                 f"pages, got {tuple(shape)} and {tuple(v_cache.shape)}")
-    if page_table.dim() != 2 or page_table.shape[0] != batch or not page_table.is_contiguous():
-        _refuse(op, f"page_table must be a contiguous int32 [{batch}, pages], got {tuple(page_table.shape)}")
+    table = page_table.shape
+    if len(table) != 2 or table[0] != batch or not page_table.is_contiguous():
+        _refuse(op, f"page_table must be a contiguous int32 [{batch}, pages], got {tuple(table)}")
     if kv_len.shape != (batch,) or not kv_len.is_contiguous():
         _refuse(op, f"kv_len must be a contiguous int32 [{batch}], got {tuple(kv_len.shape)}")
-    return strides[0] if shape[0] > 1 else shape[1] * row, shape[0], shape[1], page_table.shape[1]
+    return strides[0] if shape[0] > 1 else shape[1] * row, shape[0], shape[1], table[1]
+
+
+_raw_stream = None
 
 
 def _stream_on(dev: int, stream) -> int:
     """The given stream, or the current one of device `dev`."""
+    global _raw_stream
     if stream is not None:
         return stream.cuda_stream
-    import torch
-    return torch.cuda.current_stream(dev).cuda_stream
+    if _raw_stream is None:
+        import torch
+        # (the handle alone, where this torch has the call: current_stream() takes 1.4 us)
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                              lambda d: torch.cuda.current_stream(d).cuda_stream)
+    return _raw_stream(dev)
 
 
 def kv_append(q, k, v, k_cache, v_cache, page_table, cu_q, kv_len, n_head: int, n_kv_heads: int, head_dim: int,
@@ -441,20 +446,20 @@ def kv_append(q, k, v, k_cache, v_cache, page_table, cu_q, kv_len, n_head: int, 
     import torch
     op = "kv_append"
     dev, dtype, tokens = _device_of(op, q), q.dtype, q.shape[0]
-    batch = _bounds(op, dev, cu_q)
-    page_stride, pages, page_size, width = _cache(op, dev, dtype, k_cache, v_cache, page_table, kv_len, batch,
-                                                  n_kv_heads, head_dim)
+    batch = _bounds(op, cu_q)
     if q_out is None:
         q_out = torch.empty(tokens, n_head * head_dim, dtype=dtype, device=q.device)
-    _on(op, dev, dtype, k=k, v=v, q_out=q_out)
-    _on(op, dev, torch.float32, cos=cos, sin=sin)
+    _on(op, dev, dtype, k, v, k_cache, v_cache, q_out)
+    _on(op, dev, torch.int32, cu_q, kv_len, page_table)
+    _on(op, dev, torch.float32, cos, sin)
+    page_stride, pages, page_size, width = _cache(op, k_cache, v_cache, page_table, kv_len, batch, n_kv_heads, head_dim)
     if cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] * 2 != head_dim or not (
             cos.is_contiguous() and sin.is_contiguous()):
         _refuse(op, f"cos and sin must be contiguous [positions, {head_dim // 2}]")
     norms = [0, 0]
     for i, t in enumerate((q_norm, k_norm)):
         if t is not None:
-            _on(op, dev, torch.float32, norm=t)
+            _on(op, dev, torch.float32, t)
             if t.shape != (head_dim,) or not t.is_contiguous():
                 _refuse(op, f"norm weights must be contiguous [{head_dim}], got {tuple(t.shape)}")
             norms[i] = t.data_ptr()
@@ -481,12 +486,15 @@ def attention_paged(q, k_cache, v_cache, page_table, cu_q, kv_len, n_head: int, 
     is the longest context expected (0: the table's width), which only guides how
     the work is divided. window >= 0 lets a query see its last `window`
     positions; a query that sees none is zero."""
+    import torch
     op = "attention_paged"
-    dev, dtype, tokens = _device_of(op, q), q.dtype, q.shape[0]
-    batch = _bounds(op, dev, cu_q)
-    page_stride, pages, page_size, width = _cache(op, dev, dtype, k_cache, v_cache, page_table, kv_len, batch,
-                                                  n_kv_heads, head_dim)
-    out = _out(op, dev, q, out)
+    dev, tokens = _device_of(op, q), q.shape[0]
+    batch = _bounds(op, cu_q)
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    _on(op, dev, q.dtype, k_cache, v_cache, out)
+    _on(op, dev, torch.int32, cu_q, kv_len, page_table)
+    page_stride, pages, page_size, width = _cache(op, k_cache, v_cache, page_table, kv_len, batch, n_kv_heads, head_dim)
     args = _lib.ATTENTION_PAGED_ARGS.pack(
         q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
         _rows(op, "q", q, tokens, n_head * head_dim), _rows(op, "out", out, tokens, n_head * head_dim), tokens, batch,
@@ -505,11 +513,14 @@ def attention_packed(q, k, v, cu_seqlens, n_head: int, n_kv_heads: int, head_dim
     cu_seqlens[b+1] (int32 [batch+1]) of q [tokens, n_head*head_dim] and of k, v
     [tokens, n_kv_heads*head_dim] belong to sequence b. window >= 0: the last
     `window` keys (causal), or |t - j| <= window."""
+    import torch
     op = "attention_packed"
-    dev, dtype, tokens = _device_of(op, q), q.dtype, q.shape[0]
-    batch = _bounds(op, dev, cu_seqlens)
-    out = _out(op, dev, q, out)
-    _on(op, dev, dtype, k=k, v=v)
+    dev, tokens = _device_of(op, q), q.shape[0]
+    batch = _bounds(op, cu_seqlens)
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    _on(op, dev, q.dtype, k, v, out)
+    _on(op, dev, torch.int32, cu_seqlens)
     args = _lib.ATTENTION_PACKED_ARGS.pack(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _rows(op, "q", q, tokens, n_head * head_dim),
         _rows(op, "k", k, tokens, n_kv_heads * head_dim), _rows(op, "v", v, tokens, n_kv_heads * head_dim),
@@ -518,15 +529,6 @@ def attention_packed(q, k, v, cu_seqlens, n_head: int, n_kv_heads: int, head_dim
     rc = _lib.load().rb_attention_packed(args, _stream_on(dev, stream))
     if rc:
         _check(rc, op, tokens, batch, head_dim)
-    return out
-
-
-def _out(op: str, dev: int, q, out):
-    """The output buffer: q's shape and dtype."""
-    if out is None:
-        import torch
-        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    _on(op, dev, q.dtype, out=out)
     return out
 
 
