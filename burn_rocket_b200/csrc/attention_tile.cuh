@@ -351,17 +351,23 @@ tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
-
   // The k-th unit of this CTA: back and forth over the CTAs, so that each gets
   // early (heavy) and late (light) units alike; one a cluster when split.
   auto unit_of = [&](int k) -> int {
     if (SPLIT) return k == 0 ? static_cast<int>(blockIdx.x) / ranks : -1;
     return k * gridDim.x + ((k & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
   };
+  Finder finder;
+  Item first_item;
+  if (warp == 0) {  // the first unit is found while the block sets up
+    finder.init(p);
+    first_item = make_item(p, finder, unit_of(0), rank, ranks);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
   // Reads item k (lane 0 of a warp or a single thread waits; `arrive` once a role).
   auto get_item = [&](int k, Item& it) -> bool {
     if (!mbar_wait(&i_full[k & 1], (k >> 1) & 1, err, abort_flag)) return false;
@@ -384,10 +390,8 @@ tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
     const int page = kv.table ? 1 << kv.page_shift : 0;
     const int per_tile = kv.table ? BN >> kv.page_shift : 0;  // pages a tile
     int kv_base = 0, loaded = 0;
-    Finder finder;
-    finder.init(p);
     for (int k = 0;; ++k) {
-      const Item it = make_item(p, finder, unit_of(k), rank, ranks);
+      const Item it = k == 0 ? first_item : make_item(p, finder, unit_of(k), rank, ranks);
       if (k >= 2 && !warp_wait(&i_empty[k & 1], ((k >> 1) - 1) & 1, err, abort_flag)) break;
       if (lane == 0) {
         items[k & 1] = it;
@@ -594,12 +598,16 @@ tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
     const uint32_t s_col = s * 256, o_col = s * 256 + 128;
     const int tok = row / p.group, sub = row - tok * p.group;
     int it_n = 0, kv_base = 0;
-    Item it;
-    for (int k = 0;; ++k) {
-      if (!__all_sync(0xffffffffu, get_item(k, it))) break;
+    Item next;
+    auto take_item = [&](int k) -> bool {
+      if (!__all_sync(0xffffffffu, get_item(k, next))) return false;
       __syncwarp();
       if (lane == 0) mbar_arrive(&i_empty[k & 1]);
-      if (it.b < 0) break;
+      return true;
+    };
+    bool going = take_item(0);
+    for (int k = 0; going && next.b >= 0; ++k) {
+      const Item it = next;
       const int slo = s ? it.lo[1] : it.lo[0], shi = s ? it.hi[1] : it.hi[0];
       const int lo = max(it.ja, slo), hi = min(it.jb, shi);
       const int ia = it.i0 + s * p.tq;                // the slot's first token
@@ -747,6 +755,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
       if (!ok) break;
       kv_base += max(0, it.jb - it.ja + 1);
       const bool has = lo <= hi;
+      if (!SPLIT) going = take_item(k + 1);  // while the last P·V runs
       if (has) {
         if (!__all_sync(0xffffffffu, mbar_wait(&o_done[s], (it_n - 1) & 1, err, abort_flag))) break;
         tc_fence_after();
@@ -768,47 +777,58 @@ tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
       const bool empty = row_lo > row_hi;
       const unsigned valid_rows = __ballot_sync(0xffffffffu, valid);
       const float inv = 1.0f / l;
-      float check = 0.0f;
+      // Every column of the row at once: one TMEM latency, and the next unit's
+      // first P·V may overwrite O from here on.
+      constexpr int NCH = (D + 31) / 32;
+      uint32_t r[NCH][32];
 #pragma unroll
-      for (int c0 = 0; c0 < D; c0 += 32) {
-        uint32_t r[32];
-        tmem_ld32(lane_base + o_col + c0, r);
-        tmem_wait_ld();
-        if (c0 + 32 >= D) {  // O is out: the next unit's first P·V may overwrite it
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&o_free[s]);
-        }
+      for (int ch = 0; ch < NCH; ++ch) tmem_ld32(lane_base + o_col + 32 * ch, r[ch]);
+      tmem_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&o_free[s]);
+      uint16_t* to[4];  // the rows of this lane's four
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        to[e] = reinterpret_cast<uint16_t*>(
+            __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(out), (lane & ~3) + e));
+      const uint64_t inv2 = f2_pack(inv, inv), zero2 = f2_pack(0.0f, 0.0f);
+      uint64_t check[4] = {zero2, zero2, zero2, zero2};  // stays 0 while every value is finite
+#pragma unroll
+      for (int ch = 0; ch < NCH; ++ch) {
         uint4 w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           uint32_t u[4];
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            const float y0 = __uint_as_float(r[8 * e + 2 * q]) * inv, y1 = __uint_as_float(r[8 * e + 2 * q + 1]) * inv;
-            if (c0 + 8 * e < DH) check = fmaf(y0, 0.0f, fmaf(y1, 0.0f, check));
+            const uint64_t y = f2_mul(
+                f2_pack(__uint_as_float(r[ch][8 * e + 2 * q]), __uint_as_float(r[ch][8 * e + 2 * q + 1])), inv2);
+            if (32 * ch + 8 * e < DH) check[q] = f2_fma(y, zero2, check[q]);
+            float y0, y1;
+            f2_unpack(y, y0, y1);
             u[q] = empty ? 0u : pack2<BF16>(y0, y1);
           }
           w[e] = make_uint4(u[0], u[1], u[2], u[3]);
         }
-        if (c0 + 32 <= DH) {
+        if (32 * ch + 32 <= DH) {
           // Four lanes turn their four chunks about, so that one store covers
           // 64 contiguous bytes of eight rows instead of 16 of thirty-two.
           transpose4(w, lane);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int from = (lane & ~3) + e;
-            uint16_t* dst = reinterpret_cast<uint16_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(out), from));
-            if (valid_rows >> from & 1) *reinterpret_cast<uint4*>(dst + c0 + 8 * (lane & 3)) = w[e];
-          }
+          for (int e = 0; e < 4; ++e)
+            if (valid_rows >> ((lane & ~3) + e) & 1)
+              *reinterpret_cast<uint4*>(to[e] + 32 * ch + 8 * (lane & 3)) = w[e];
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (valid && c0 + 8 * e < DH) *reinterpret_cast<uint4*>(out + c0 + 8 * e) = w[e];
+            if (valid && 32 * ch + 8 * e < DH) *reinterpret_cast<uint4*>(out + 32 * ch + 8 * e) = w[e];
         }
       }
+      float c0, c1;
+      f2_unpack(f2_add(f2_add(check[0], check[1]), f2_add(check[2], check[3])), c0, c1);
       __syncwarp();  // before the mark: other lanes stored parts of the row
-      if (valid && !empty && !(check == 0.0f)) {  // marked by a NaN of either type
+      if (valid && !empty && !(c0 + c1 == 0.0f)) {  // marked by a NaN of either type
         *reinterpret_cast<uint32_t*>(out) = 0x7fff7fffu;
         redo[0] = 1;
       }
