@@ -777,16 +777,6 @@ tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
       const bool empty = row_lo > row_hi;
       const unsigned valid_rows = __ballot_sync(0xffffffffu, valid);
       const float inv = 1.0f / l;
-      // Every column of the row at once: one TMEM latency, and the next unit's
-      // first P·V may overwrite O from here on.
-      constexpr int NCH = (D + 31) / 32;
-      uint32_t r[NCH][32];
-#pragma unroll
-      for (int ch = 0; ch < NCH; ++ch) tmem_ld32(lane_base + o_col + 32 * ch, r[ch]);
-      tmem_wait_ld();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&o_free[s]);
       uint16_t* to[4];  // the rows of this lane's four
 #pragma unroll
       for (int e = 0; e < 4; ++e)
@@ -794,37 +784,42 @@ tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
             __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(out), (lane & ~3) + e));
       const uint64_t inv2 = f2_pack(inv, inv), zero2 = f2_pack(0.0f, 0.0f);
       uint64_t check[4] = {zero2, zero2, zero2, zero2};  // stays 0 while every value is finite
-#pragma unroll
-      for (int ch = 0; ch < NCH; ++ch) {
+      // Not unrolled: this code runs once a unit, and each of its instructions is
+      // fetched anew.
+#pragma unroll 1
+      for (int at = 0; at < DH; at += 32) {
+        uint32_t r[32];
+        tmem_ld32(lane_base + o_col + at, r);
+        tmem_wait_ld();
         uint4 w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           uint32_t u[4];
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            const uint64_t y = f2_mul(
-                f2_pack(__uint_as_float(r[ch][8 * e + 2 * q]), __uint_as_float(r[ch][8 * e + 2 * q + 1])), inv2);
-            if (32 * ch + 8 * e < DH) check[q] = f2_fma(y, zero2, check[q]);
+            const uint64_t y =
+                f2_mul(f2_pack(__uint_as_float(r[8 * e + 2 * q]), __uint_as_float(r[8 * e + 2 * q + 1])), inv2);
+            if (DH % 32 == 0 || at + 8 * e < DH) check[q] = f2_fma(y, zero2, check[q]);
             float y0, y1;
             f2_unpack(y, y0, y1);
             u[q] = empty ? 0u : pack2<BF16>(y0, y1);
           }
           w[e] = make_uint4(u[0], u[1], u[2], u[3]);
         }
-        if (32 * ch + 32 <= DH) {
+        if (DH % 32 == 0 || at + 32 <= DH) {
           // Four lanes turn their four chunks about, so that one store covers
           // 64 contiguous bytes of eight rows instead of 16 of thirty-two.
           transpose4(w, lane);
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (valid_rows >> ((lane & ~3) + e) & 1)
-              *reinterpret_cast<uint4*>(to[e] + 32 * ch + 8 * (lane & 3)) = w[e];
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (valid && 32 * ch + 8 * e < DH) *reinterpret_cast<uint4*>(out + 32 * ch + 8 * e) = w[e];
+            if (valid_rows >> ((lane & ~3) + e) & 1) *reinterpret_cast<uint4*>(to[e] + at + 8 * (lane & 3)) = w[e];
+        } else if (valid) {
+          *reinterpret_cast<uint4*>(out + at) = w[0];  // the last 8 columns of a 72-wide head
         }
       }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&o_free[s]);  // the next unit's first P·V may overwrite O
       float c0, c1;
       f2_unpack(f2_add(f2_add(check[0], check[1]), f2_add(check[2], check[3])), c0, c1);
       __syncwarp();  // before the mark: other lanes stored parts of the row
