@@ -255,9 +255,13 @@ static std::atomic<int64_t> g_launches{0};
 
 static int ensure_engine(Engine** out) {
   if (!g_engine) return fail(RB_E_IO, "rb_init() has not been called");
+  // A thread that has made no runtime call yet has no current context, which
+  // encoding a tensor map needs: its first call sets the device all the same.
+  static thread_local bool bound = false;
   int cur = -1;
   cudaGetDevice(&cur);
-  if (cur != g_engine->device) RB_CUDA(cudaSetDevice(g_engine->device), "cudaSetDevice");
+  if (cur != g_engine->device || !bound) RB_CUDA(cudaSetDevice(g_engine->device), "cudaSetDevice");
+  bound = true;
   *out = g_engine;
   return RB_OK;
 }

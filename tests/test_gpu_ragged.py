@@ -148,6 +148,14 @@ PAGED = [
     ([200, 131], [1500, 131], 14, 2, 128, 16, 150, 0.0),
     ([40, 257], [640, 257], 8, 1, 64, 32, -1, 20.0),
     ([500, 1, 1], [4100, 2000, 1], 4, 4, 64, 64, -1, 0.0),
+    # more sequences than the GPU holds at once (with equal lengths among them), than a warp ranks
+    ([1] * 70, [1 + (37 * i) % 300 for i in range(70)], 16, 8, 128, 16, -1, 0.0),
+    ([1] * 150, [1 + (11 * i) % 90 for i in range(150)], 8, 8, 64, 32, 40, 0.0),
+    ([2, 20] * 70, [30, 50] * 70, 8, 1, 64, 16, -1, 0.0),
+    ([40] + [1] * 30, [200] + [5 * i + 1 for i in range(30)], 16, 8, 128, 64, -1, 0.0),
+    # many query heads a KV head
+    ([1, 3], [200, 40], 32, 1, 128, 16, -1, 0.0),
+    ([1, 2], [130, 300], 128, 1, 64, 128, -1, 0.0),
     # more new tokens than keys: the first rows stand before position 0 and see nothing
     ([9, 150], [4, 100], 16, 8, 128, 16, -1, 0.0),
     ([2, 1], [1, 0], 4, 1, 64, 16, -1, 0.0),
@@ -195,6 +203,10 @@ PACKED = [
     ([255, 300], 6, 2, 72, False, 128, 0.0),
     ([1500], 4, 2, 128, True, -1, 0.0),
     ([20] * 40, 16, 8, 128, True, -1, 0.0),
+    ([3, 0, 70] * 60, 4, 2, 64, True, -1, 0.0),
+    ([3, 70] * 70, 4, 2, 64, False, -1, 0.0),
+    ([129, 5], 128, 1, 64, True, -1, 0.0),
+    ([700, 2, 300, 300], 4, 1, 128, False, 500, 0.0),
 ]
 
 
@@ -549,6 +561,78 @@ def test_graph_replays_with_new_lengths(rb, n):
     a.k, a.v = [a.k[0][:130 + n], a.k[1][:0]], [a.v[0][:130 + n], a.v[1][:0]]
     a.verify(outs[0])
     rb.check_device_errors()
+
+
+FIRST_CALL = """
+import sys, math
+sys.path.insert(0, {root!r})
+import torch
+import burn_rocket_b200 as rb
+rb.init(0)
+h, hkv, d, page, dt = 4, 2, 128, 16, torch.float16
+lens = torch.tensor([200, 90], dtype=torch.int32, device="cuda")
+for n in (1, 60):
+    q = torch.randn(2 * n, h * d, device="cuda").to(dt)
+    kv = torch.randn(2 * n, hkv * d, device="cuda").to(dt)
+    k_cache, v_cache = (torch.randn(30, page, hkv, d, device="cuda").to(dt) for _ in range(2))
+    table = torch.randperm(30, device="cuda")[:28].view(2, 14).to(torch.int32)
+    cu = torch.arange(3, device="cuda", dtype=torch.int32) * n
+    cos, sin = torch.randn(2, 256, d // 2, device="cuda").unbind()
+    def step():
+        r = rb.kv_append(q, kv, kv, k_cache, v_cache, table, cu, lens, h, hkv, d, cos, sin)
+        return rb.attention_paged(r, k_cache, v_cache, table, cu, lens, h, hkv, d, 0.1, max_q=n), \\
+            rb.attention_packed(r, kv, kv, cu, h, hkv, d, 0.1)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = step()
+    g.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(outs, step()):
+        assert torch.isfinite(a).all() and torch.equal(a, b)
+rb.check_device_errors()
+print("captured first")
+"""
+
+
+def test_first_call_may_be_a_capture():
+    """Nothing is set up outside the stream that a capture would refuse: the
+    first call of a process can be the captured one."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    root = str(Path(__file__).resolve().parent.parent)
+    run = subprocess.run([sys.executable, "-c", FIRST_CALL.format(root=root)], capture_output=True, text=True, timeout=120)
+    assert run.returncode == 0 and "captured first" in run.stdout, run.stderr[-2000:]
+
+
+def test_calls_at_the_same_time(rb):
+    """Threads and streams share nothing: each gets its own result."""
+    import threading
+    batches = [Batch([n, n], [m, m // 2 + n], 16, 8, 128, 16, torch.bfloat16, seed=i)
+               for i, (n, m) in enumerate([(1, 3000), (70, 700), (1, 90), (200, 500)])]
+    outs = [torch.full_like(b.q, 7.0) for b in batches]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(b, out):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    b.attend(rb, out=out)
+        except Exception as e:  # noqa: BLE001 (reported below)
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=x) for x in zip(batches, outs)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    torch.cuda.synchronize()
+    rb.check_device_errors()
+    assert not failed
+    for b, out in zip(batches, outs):
+        b.verify(out)
 
 
 def test_streams_and_views(rb):
