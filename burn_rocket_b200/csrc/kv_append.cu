@@ -10,17 +10,19 @@
 //
 // One read of q, k, v and one write each: HBM bound, and for a few tokens the
 // chain of dependent loads (sequence bounds -> its lengths -> page id and
-// angles) is all there is. A warp takes up to kPasses * 512 / D heads of one
-// token; lane groups of D/16 lanes hold a head, each lane eight elements of
-// either half (16-byte accesses), and the whole share's loads are issued
-// before the chain is walked.
+// angles) is all there is. A warp takes 2 or 3 passes of 512 / D heads of one
+// token, whichever wastes fewer lanes (more on a tie); lane groups of D/16 lanes
+// hold a head, each lane eight elements of either half (16-byte accesses), and
+// the whole share's loads are issued before the chain is walked. Six blocks an SM
+// hide the chain: 4 passes at 108 registers took 59 us for 23238 tokens of 32/4 x
+// 64 bf16 heads without a norm (238 MB), 3 at 80 registers 47 us (5.1 TB/s), 2 50;
+// 16/8 x 128 f16 heads with norms 57, 60 and 56 us (263 MB, 4.7 TB/s); one decode
+// token of 32 sequences 4.2, 4.3 and 3.6.
 #include "ragged.cuh"
 
 namespace rb {
 
 namespace append {
-
-constexpr int kPasses = 4;
 
 __device__ __forceinline__ void unpack8(const uint4& u, bool bf16, float (&f)[8]) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -56,8 +58,8 @@ __device__ __forceinline__ void load8(const float* p, float (&f)[8]) {
   f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
 }
 
-template <int D, bool BF16>
-__global__ void __launch_bounds__(128) kv_append_kernel(const KvAppend p, int shares) {
+template <int D, bool BF16, int PASSES>
+__global__ void __launch_bounds__(128, 6) kv_append_kernel(const KvAppend p, int shares) {
   constexpr int LH = D / 16;       // lanes a head
   constexpr int HP = 32 / LH;      // heads a pass
   const int lane = threadIdx.x & 31;
@@ -66,10 +68,10 @@ __global__ void __launch_bounds__(128) kv_append_kernel(const KvAppend p, int sh
   if (t >= p.seqs.tokens) return;
   const int units = p.n_head + 2 * p.n_kv_heads;  // q heads, k heads, v heads
   const int col = 8 * (lane % LH);
-  uint4 lo[kPasses], hi[kPasses];
+  uint4 lo[PASSES], hi[PASSES];
 #pragma unroll
-  for (int i = 0; i < kPasses; ++i) {
-    const int u = (share * kPasses + i) * HP + lane / LH;
+  for (int i = 0; i < PASSES; ++i) {
+    const int u = (share * PASSES + i) * HP + lane / LH;
     lo[i] = hi[i] = make_uint4(0u, 0u, 0u, 0u);
     if (u >= units) continue;
     const uint16_t* src = u < p.n_head ? p.q + t * p.ldq + u * D
@@ -93,8 +95,8 @@ __global__ void __launch_bounds__(128) kv_append_kernel(const KvAppend p, int sh
   load8(p.cos_t + static_cast<int64_t>(pos) * (D / 2) + col, c8);
   load8(p.sin_t + static_cast<int64_t>(pos) * (D / 2) + col, s8);
 #pragma unroll
-  for (int i = 0; i < kPasses; ++i) {
-    const int u = (share * kPasses + i) * HP + lane / LH;
+  for (int i = 0; i < PASSES; ++i) {
+    const int u = (share * PASSES + i) * HP + lane / LH;
     const bool is_q = u < p.n_head, is_k = !is_q && u < p.n_head + p.n_kv_heads;
     float a[8], c[8];
     unpack8(lo[i], BF16, a);
@@ -136,16 +138,22 @@ __global__ void __launch_bounds__(128) kv_append_kernel(const KvAppend p, int sh
   }
 }
 
-template <int D>
-static int launch(const KvAppend& a, cudaStream_t st) {
-  constexpr int per = kPasses * 512 / D;  // heads a warp
-  const int shares = (a.n_head + 2 * a.n_kv_heads + per - 1) / per;
+template <int D, int PASSES>
+static int launch(const KvAppend& a, int passes, cudaStream_t st) {
+  const int shares = (passes + PASSES - 1) / PASSES;
   const int64_t blocks = (static_cast<int64_t>(a.seqs.tokens) * shares + 3) / 4;
-  if (blocks > 0x7fffffff) return RB_E_SHAPE;
-  if (a.bf16) kv_append_kernel<D, true><<<static_cast<unsigned>(blocks), 128, 0, st>>>(a, shares);
-  else kv_append_kernel<D, false><<<static_cast<unsigned>(blocks), 128, 0, st>>>(a, shares);
+  if (blocks > 0x7fffffff) return report_error(RB_E_SHAPE, "kv_append: too many tokens");
+  if (a.bf16) kv_append_kernel<D, true, PASSES><<<static_cast<unsigned>(blocks), 128, 0, st>>>(a, shares);
+  else kv_append_kernel<D, false, PASSES><<<static_cast<unsigned>(blocks), 128, 0, st>>>(a, shares);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? RB_OK : report_error(RB_E_DEVICE, cudaGetErrorString(e));
+}
+
+template <int D>
+static int launch(const KvAppend& a, cudaStream_t st) {
+  constexpr int HP = 512 / D;  // heads a pass
+  const int passes = (a.n_head + 2 * a.n_kv_heads + HP - 1) / HP;
+  return (passes + 2) / 3 * 3 <= (passes + 1) / 2 * 2 ? launch<D, 3>(a, passes, st) : launch<D, 2>(a, passes, st);
 }
 
 }  // namespace append
