@@ -5,6 +5,7 @@
 // the caller's stream that touch only the caller's buffers and the engine's
 // error word, so calls may run at the same time on any streams and inside
 // graphs.
+#include <algorithm>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -224,7 +225,7 @@ extern "C" int rb_attention_packed(const rb_attention_packed_args* args, void* s
   AttnRagged a{};
   a.seqs = {cu_seqlens, nullptr, static_cast<int>(batch), static_cast<int>(tokens), static_cast<int>(tokens),
             static_cast<int>(tokens), e.err};
-  a.hint_kv = static_cast<int>(tokens);
+  a.hint_kv = static_cast<int>(batch == 1 ? tokens : std::min(tokens, 2 * tokens / batch + 1));  // twice the mean
   a.kv.k = static_cast<const uint16_t*>(k);
   a.kv.v = static_cast<const uint16_t*>(v);
   a.kv.ldk = ldk;

@@ -68,6 +68,11 @@ def test_attention_packed_refuses(change):
     assert _lib.last_error().startswith("attention_packed:")
 
 
+def test_null_arguments_are_refused():
+    for name in ("rb_kv_append", "rb_attention_paged", "rb_attention_packed"):
+        assert getattr(_lib.load(), name)(None, None) == _lib.RB_E_SHAPE
+
+
 @pytest.mark.parametrize("name,base", [("rb_kv_append", APPEND), ("rb_attention_paged", PAGED),
                                        ("rb_attention_packed", PACKED)])
 def test_empty_batches_are_no_work(name, base):
