@@ -25,6 +25,14 @@
 //   * split: where there are fewer units than SMs, a cluster of CTAs takes equal
 //     runs of one unit's key tiles and merges (O, m, l) through distributed
 //     shared memory: no workspace in global memory.
+//
+// Bound: a slot's chain per 128 keys, about 3400 clocks (TMEM load 180, maximum
+// 200, exponentials and P stores 1430 of which the MUFU needs 1024, store wait
+// 170, P·V and the next S 1400), beside 2048 of UMMA for both slots: tensor pipe
+// 48% active. 8 x 2048 tokens causal, 32/4 heads x 128: 287 us, 957 TFLOP/s; 64 x
+// 512 causal, 16/8 heads: 132 us (the dense kernel 205); 16 x 2394 bidirectional,
+// 16 heads x 72: 652 us (dense 822); a unit of one or two key tiles pays as much
+// again to start and end.
 #pragma once
 
 #include <algorithm>
@@ -40,7 +48,9 @@ constexpr int BM = 128;  // rows of a slot
 constexpr int BN = 128;  // keys of a tile
 // Three warpgroups: warps 0-3 (TMA, UMMA, two idle), 4-7 and 8-11 (softmax of
 // slot 0 and 1). The block starts with kLaunchRegs a thread; the first warpgroup
-// hands registers to the other two, whose 128 scores a row do not fit 168.
+// hands registers to the other two, whose 128 scores a row do not fit 168 (with
+// 150 to 250 bytes of spills 64 x 512 causal took 204 us, without 148; 88 / 208
+// already spills in the first warpgroup).
 constexpr int kThreads = 12 * 32;
 constexpr int kSoftWarp0 = 4;
 constexpr int kSoftThreads = 8 * 32;
