@@ -83,7 +83,12 @@ __global__ void __launch_bounds__(128, 6) kv_append_kernel(const KvAppend p, int
   const int b = find_seq(p.seqs.cu, p.seqs.batch, t);
   if (b < 0) return;  // a row behind the last sequence
   const Seq s = load_seq(p.seqs, b);
-  if (t - s.q0 >= s.n) return;  // a skipped sequence
+  // A skipped sequence, or bounds that fall: then the search can end at a
+  // sequence on either side of the row.
+  if (t < s.q0 || t - s.q0 >= s.n) {
+    atomicOr(p.seqs.err, kErrBadShape);
+    return;
+  }
   const int pos = s.kv - s.n + t - s.q0;
   if (pos < 0 || pos >= p.max_pos) {
     atomicOr(p.seqs.err, kErrBadShape);

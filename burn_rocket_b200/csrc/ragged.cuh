@@ -39,9 +39,10 @@ __device__ __forceinline__ Seq load_seq(const RaggedBatch& r, int b) {
   return s;
 }
 
-// Sequence that owns token row t (cu is non-decreasing), or -1 for a row
-// outside every sequence. One warp: each step reads 32 evenly spaced bounds at
-// once, so 32768 sequences take three dependent loads.
+// Sequence that owns token row t, or -1 for a row outside every sequence. One
+// warp: each step reads 32 evenly spaced bounds at once, so 32768 sequences take
+// three dependent loads. Where the bounds fall, against the contract, the result
+// may be a sequence that does not hold the row: the caller compares.
 __device__ __forceinline__ int find_seq(const int32_t* cu, int batch, int t) {
   const int lane = threadIdx.x & 31;
   int lo = 0, hi = batch;  // the answer is the number of b in [0, batch] with cu[b] <= t, less one

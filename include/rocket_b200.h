@@ -257,7 +257,10 @@ RB_API int rb_attention_batched(const void* q, int64_t ldq, const void* k, int64
  * outside the token rows, more keys than the table has slots, more than max_q
  * tokens or (rb_kv_append) a position outside the angle table is skipped, a page
  * id outside the cache is not followed (its keys and values read as zeros, its
- * tokens are not stored), and rb_check_device_errors reports bad-shape.
+ * tokens are not stored), and rb_check_device_errors reports bad-shape. Bounds
+ * that fall are reported too: a row that several sequences claim then holds any
+ * one's attention, and rb_kv_append leaves out the rows whose sequence its search
+ * does not find; it stores a row in no other sequence's slots.
  *
  * Arguments are structures (many, and cheap to pass through a binding); every
  * field is read before the call returns. The calls allocate nothing and share no workspace: they may run at the same

@@ -680,3 +680,38 @@ def test_wrapper_refusals(rb):
         with pytest.raises(rb.OpFailure):
             rb.attention_packed(*bad, 4, 4, 128, 0.1)
     rb.check_device_errors()
+
+
+@pytest.mark.parametrize("cu", [[0, 6, 8, 2, 9], [0, 8, 9, 4, 12], [0, 2, 1, 4], [0, 5, 3, 9, 7, 12]])
+def test_append_with_falling_bounds(rb, cu):
+    """Where bounds fall, a row goes only to a slot of a sequence that holds the
+    row; every other row is skipped, every other slot stays as it was, and it is
+    reported."""
+    h, hkv, d, page = 2, 2, 64, 16
+    n, kv = len(cu) - 1, [30 + 9 * i for i in range(len(cu) - 1)]
+    b = Batch([cu[-1]] + [0] * (n - 1), kv, h, hkv, d, page, torch.bfloat16, tail_rows=0)
+    b.cu = torch.tensor(cu, device="cuda", dtype=torch.int32)
+    cos, sin = torch.ones(128, d // 2, device="cuda"), torch.zeros(128, d // 2, device="cuda")
+    q_out = torch.full_like(b.q, 7.0)
+    new = torch.randn(cu[-1], hkv * d, device="cuda").bfloat16()
+    before = b.k_cache.clone(), b.v_cache.clone()
+    rb.kv_append(b.q, new, new, b.k_cache, b.v_cache, b.table, b.cu, b.kv_len, h, hkv, d, cos, sin, q_out=q_out)
+    with pytest.raises(rb.OpFailure, match="bad-shape"):
+        rb.check_device_errors()
+    stored = (q_out != 7.0).any(-1).tolist()
+    bits = torch.int16
+    for cache, was in zip((b.k_cache, b.v_cache), before):
+        want, found = was.clone(), 0
+        for t in range(cu[-1]):
+            for s in range(n):
+                if cu[s] <= t < cu[s + 1]:
+                    pos = kv[s] - (cu[s + 1] - cu[s]) + t - cu[s]
+                    at = b.table[s, pos // page].long(), pos % page
+                    if stored[t] and torch.equal(cache[at], new[t].view(hkv, d)):
+                        want[at] = cache[at]
+                        found += 1
+        assert found == sum(stored)
+        assert torch.equal(cache.contiguous().view(bits), want.contiguous().view(bits))
+    for t in range(cu[-1]):
+        assert not stored[t] or torch.equal(q_out[t], b.q[t])
+    assert stored[0] and not all(stored)  # row 0 lies in the first sequence alone
