@@ -89,11 +89,11 @@ __global__ void __launch_bounds__(128, 6) kv_append_kernel(const KvAppend p, int
     atomicOr(p.seqs.err, kErrBadShape);
     return;
   }
-  const int pos = s.kv - s.n + t - s.q0;
-  if (pos < 0 || pos >= p.max_pos) {
+  if (s.kv < s.n || s.kv > p.max_pos) {  // a position outside the angle table: none of the sequence's tokens
     atomicOr(p.seqs.err, kErrBadShape);
     return;
   }
+  const int pos = s.kv - s.n + t - s.q0;
   const int64_t slot = slot_offset(p.cache, b, pos, p.seqs.err);
   if (slot < 0) return;
   float c8[8], s8[8];

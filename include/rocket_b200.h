@@ -253,18 +253,20 @@ RB_API int rb_attention_batched(const void* q, int64_t ldq, const void* k, int64
  * page_table[b*ld_table + j/page_size]. Table entries past a sequence's last
  * page are not read, slots past its last position may hold anything.
  *
- * What the device data says is checked on the device: a sequence with bounds
- * outside the token rows, more keys than the table has slots, more than max_q
- * tokens or (rb_kv_append) a position outside the angle table is skipped, a page
- * id outside the cache is not followed (its keys and values read as zeros, its
- * tokens are not stored), and rb_check_device_errors reports bad-shape. Bounds
- * that fall are reported too: a row that several sequences claim then holds any
- * one's attention, and rb_kv_append leaves out the rows whose sequence its search
- * does not find; it stores a row in no other sequence's slots.
+ * What the device data says is checked on the device, and what does not fit is
+ * reported by rb_check_device_errors (bad-shape): a sequence with bounds outside
+ * the token rows, more keys than the table has slots, more than max_q tokens or
+ * (rb_kv_append) a position before 0 or past the angle table is skipped whole; a
+ * page id outside the cache is not followed (its keys and values read as zeros,
+ * its tokens are neither stored nor rotated). Where the bounds fall, a row that
+ * several sequences claim holds any one's attention, and rb_kv_append leaves out
+ * the rows that its search does not find in a sequence; it stores a row in no
+ * other sequence's slots.
  *
  * Arguments are structures (many, and cheap to pass through a binding); every
- * field is read before the call returns. The calls allocate nothing and share no workspace: they may run at the same
- * time on several streams and in several graphs. */
+ * field is read before the call returns. The calls allocate nothing and share no
+ * workspace: they may run at the same time on several streams and in several
+ * graphs. */
 
 /* Appends the new tokens of each sequence to the cache: token i of sequence b
  * has position kv_len[b] - n_b + i (kv_len counts the new tokens, which are

@@ -715,3 +715,29 @@ def test_append_with_falling_bounds(rb, cu):
     for t in range(cu[-1]):
         assert not stored[t] or torch.equal(q_out[t], b.q[t])
     assert stored[0] and not all(stored)  # row 0 lies in the first sequence alone
+
+
+@pytest.mark.parametrize("n,kv,positions", [(2, 26, 25), (3, 2, 64), (40, 70, 69), (40, 39, 64), (40, 70, 70)])
+def test_append_takes_a_sequence_whole_or_not_at_all(rb, n, kv, positions):
+    """Positions that begin inside the angle table and end outside it (or begin
+    before 0): none of the sequence's tokens is stored, the other's are."""
+    h, hkv, d, page = 2, 2, 64, 16
+    b = Batch([n, 2], [kv, 20], h, hkv, d, page, torch.bfloat16, tail_rows=0)
+    fits = kv <= positions and n <= kv
+    cos, sin = torch.ones(positions, d // 2, device="cuda"), torch.zeros(positions, d // 2, device="cuda")
+    q_out = torch.full_like(b.q, 7.0)
+    new = torch.randn(n + 2, hkv * d, device="cuda").bfloat16()
+    want = b.k_cache.clone(), b.v_cache.clone()
+    rb.kv_append(b.q, new, new, b.k_cache, b.v_cache, b.table, b.cu, b.kv_len, h, hkv, d, cos, sin, q_out=q_out)
+    if fits:
+        rb.check_device_errors()
+    else:
+        with pytest.raises(rb.OpFailure, match="bad-shape"):
+            rb.check_device_errors()
+    rows = ([(t, 0, kv - n + t) for t in range(n)] if fits else []) + [(n, 1, 18), (n + 1, 1, 19)]
+    for cache, was in zip((b.k_cache, b.v_cache), want):
+        for t, s, pos in rows:
+            was[b.table[s, pos // page].long(), pos % page] = new[t].view(hkv, d)
+        assert torch.equal(cache.contiguous().view(torch.int16), was.contiguous().view(torch.int16))
+    assert torch.equal(q_out[n:], b.q[n:])
+    assert torch.equal(q_out[:n], b.q[:n]) if fits else (q_out[:n] == 7.0).all()
