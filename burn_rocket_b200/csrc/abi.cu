@@ -304,7 +304,6 @@ int engine_view(EngineView* v) {
   Engine* e;
   const int rc = ensure_engine(&e);
   if (rc) return rc;
-  v->device = e->device;
   v->num_sms = e->num_sms;
   v->err = e->err;
   return RB_OK;

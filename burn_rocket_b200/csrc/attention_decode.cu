@@ -144,30 +144,28 @@ __device__ __forceinline__ int ranked_sequence(const RaggedBatch& q, int r) {
   return b;
 }
 
-// Grid: ((sequence * row tiles + row tile) * KV heads + KV head) * cluster
-// size + rank; neighbouring clusters read neighbouring heads of the same slots.
-// Where the grid is more than the GPU holds at a time, `longest_first` sends the
-// long sequences ahead.
+// Grid: (sequence * KV heads + KV head) * cluster size + rank; neighbouring
+// clusters read neighbouring heads of the same slots. Where the grid is more than
+// the GPU holds at a time, `longest_first` sends the long sequences ahead.
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kWarps * 32, 2) decode_kernel(const __grid_constant__ AttnRagged p, int row_tiles, bool longest_first) {
+__global__ void __launch_bounds__(kWarps * 32, 2) decode_kernel(const __grid_constant__ AttnRagged p, bool longest_first) {
   using G = Geo<D>;
   extern __shared__ __align__(128) uint8_t smem[];
   const uint32_t ranks = cluster_size(), rank = cluster_ctarank();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int unit = blockIdx.x / ranks;
   const int head_kv = unit % p.n_kv_heads;
-  const int tile = unit / p.n_kv_heads % row_tiles;
-  int b = unit / p.n_kv_heads / row_tiles;
+  int b = unit / p.n_kv_heads;
   if (longest_first) b = ranked_sequence(p.seqs, b);
   const int group = p.n_head / p.n_kv_heads;
   const Seq s = load_seq(p.seqs, b);
-  const int row0 = tile * kRows, rows = min(kRows, s.n * group - row0);
+  const int rows = s.n * group;  // at most kRows: load_seq skips more tokens than the launch has room for
   if (rows <= 0) return;  // the whole cluster
   const int first_pos = s.kv - s.n;  // position of the sequence's first new token
-  // Keys that any row of the tile sees, and those that every row sees.
+  // Keys that any row sees, and those that every row sees.
   int lo, hi, lo_all, hi_all;
-  visible(first_pos + row0 / group, s.kv, p.dlo, p.dhi, lo, hi_all);
-  visible(first_pos + (row0 + rows - 1) / group, s.kv, p.dlo, p.dhi, lo_all, hi);
+  visible(first_pos, s.kv, p.dlo, p.dhi, lo, hi_all);
+  visible(first_pos + s.n - 1, s.kv, p.dlo, p.dhi, lo_all, hi);
   const int block0 = lo / kRows, blocks = hi < lo ? 0 : hi / kRows - block0 + 1;
 
   // Q fragments: rows g and g + 8, columns 16 k + 2 t (+ 8).
@@ -176,7 +174,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) decode_kernel(const __grid_con
   int row_lo[2], row_hi[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const int r = row0 + g + 8 * h, i = r / group;
+    const int r = g + 8 * h, i = r / group;
     const bool there = g + 8 * h < rows;
     const uint16_t* q = p.q + (there ? static_cast<int64_t>(s.q0 + i) * p.ldq + (head_kv * group + r % group) * D : 0);
 #pragma unroll
@@ -366,7 +364,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) decode_kernel(const __grid_con
       acc = fmaf(a, ld_cluster(mapa_shared(parts + (kWarps * kRows + r) * D + col, w)), acc);
       sum = fmaf(a, all[w * 2 * kRows + kRows + r], sum);
     }
-    const int i = (row0 + r) / group, head = head_kv * group + (row0 + r) % group;
+    const int i = r / group, head = head_kv * group + r % group;
     int rl, rh;
     visible(first_pos + i, s.kv, p.dlo, p.dhi, rl, rh);
     const float y = rl > rh ? 0.0f : acc / sum;
@@ -378,7 +376,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) decode_kernel(const __grid_con
   const int again = *redo;
   for (int r = warp; r < rows; r += kWarps)
     if (again >> r & 1)
-      row_attention<D, BF16, true>(p, b, s, (row0 + r) / group, head_kv * group + (row0 + r) % group, c0, c1);
+      row_attention<D, BF16, true>(p, b, s, r / group, head_kv * group + r % group, c0, c1);
 }
 
 // Cluster size for one call. Measured on this kernel (flushed L2): a CTA alone
@@ -406,7 +404,7 @@ static int pick_ranks(const int* active, int64_t units, int batch, double keys, 
 }
 
 template <int D, bool BF16>
-static int launch(const AttnRagged& a, int row_tiles, cudaStream_t st) {
+static int launch(const AttnRagged& a, cudaStream_t st) {
   auto kernel = decode_kernel<D, BF16>;
   static std::atomic<int> resident[64][17];  // clusters of each size that a device holds; [0]: known
   int dev = 0;
@@ -436,7 +434,7 @@ static int launch(const AttnRagged& a, int row_tiles, cudaStream_t st) {
   }
   int active[17];
   for (int r = 1; r <= 16; ++r) active[r] = resident[dev][r].load(std::memory_order_relaxed);
-  const int64_t units = static_cast<int64_t>(a.seqs.batch) * a.n_kv_heads * row_tiles;
+  const int64_t units = static_cast<int64_t>(a.seqs.batch) * a.n_kv_heads;
   const int keys = a.dlo <= -kRaggedNoBound ? a.hint_kv : std::min(a.hint_kv, a.seqs.max_q - a.dlo);
   const int ranks = pick_ranks(active, units, a.seqs.batch, std::max(keys, 1), D);
   if (units * ranks > 0x7fffffff) return report_error(RB_E_SHAPE, "attention_paged: batch too large");
@@ -445,7 +443,7 @@ static int launch(const AttnRagged& a, int row_tiles, cudaStream_t st) {
   cfg.stream = st;
   at[0].val.clusterDim.x = ranks;
   cfg.numAttrs = ranks > 1 ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, row_tiles, longest_first);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, longest_first);
   return e == cudaSuccess ? RB_OK : report_error(RB_E_DEVICE, cudaGetErrorString(e));
 }
 
@@ -453,10 +451,10 @@ static int launch(const AttnRagged& a, int row_tiles, cudaStream_t st) {
 
 int launch_attention_decode(const AttnRagged& a, cudaStream_t st) {
   using namespace decode;
-  const int group = a.n_head / a.n_kv_heads;
-  const int row_tiles = static_cast<int>((static_cast<int64_t>(a.seqs.max_q) * group + kRows - 1) / kRows);
-  if (a.head_dim == 128) return a.bf16 ? launch<128, true>(a, row_tiles, st) : launch<128, false>(a, row_tiles, st);
-  return a.bf16 ? launch<64, true>(a, row_tiles, st) : launch<64, false>(a, row_tiles, st);
+  if (static_cast<int64_t>(a.seqs.max_q) * (a.n_head / a.n_kv_heads) > kRows)
+    return report_error(RB_E_SHAPE, "attention_paged: too many rows for the few-row kernel");
+  if (a.head_dim == 128) return a.bf16 ? launch<128, true>(a, st) : launch<128, false>(a, st);
+  return a.bf16 ? launch<64, true>(a, st) : launch<64, false>(a, st);
 }
 
 }  // namespace rb

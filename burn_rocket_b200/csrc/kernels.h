@@ -196,7 +196,7 @@ struct AttnRagged {
   int num_sms;
 };
 int launch_attention_ragged(const AttnRagged& a, cudaStream_t st);
-int launch_attention_decode(const AttnRagged& a, cudaStream_t st);  // paged, few rows a sequence
+int launch_attention_decode(const AttnRagged& a, cudaStream_t st);  // paged, max_q * group at most 16
 
 struct KvAppend {
   RaggedBatch seqs;
@@ -272,7 +272,6 @@ struct W8A8View {
   int device;
 };
 struct EngineView {
-  int device;
   int num_sms;
   uint32_t* err;
 };

@@ -1,10 +1,9 @@
 // ragged_abi.cu — entry points of the ragged-batch operators: argument checks
 // and the launch structures of kv_append.cu and attention_ragged.cu.
 //
-// Nothing here keeps state or allocates: every call is one or two kernels on
-// the caller's stream that touch only the caller's buffers and the engine's
-// error word, so calls may run at the same time on any streams and inside
-// graphs.
+// Nothing here keeps state or allocates: every call is one kernel on the
+// caller's stream that touches only the caller's buffers and the engine's error
+// word, so calls may run at the same time on any streams and inside graphs.
 #include <algorithm>
 #include <cmath>
 #include <cstdarg>
