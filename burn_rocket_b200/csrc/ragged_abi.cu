@@ -167,7 +167,7 @@ extern "C" int rb_attention_paged(const rb_attention_paged_args* args, void* str
       (rc = check_softmax(op, scale, softcap)) != RB_OK)
     return rc;
   if (max_q < 0 || max_kv < 0) return refuse(RB_E_SHAPE, "%s: max_q=%lld max_kv=%lld", op, (long long)max_q, (long long)max_kv);
-  if (tokens == 0 || batch == 0 || max_q == 0) return RB_OK;
+  if (tokens == 0 || batch == 0) return RB_OK;
   if ((rc = check_rows(op, "q", q, ldq, n_head, head_dim)) != RB_OK ||
       (rc = check_rows(op, "out", out, ldo, n_head, head_dim)) != RB_OK)
     return rc;

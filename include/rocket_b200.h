@@ -301,8 +301,9 @@ RB_API int rb_kv_append(const rb_kv_append_args* args, void* stream);
  * (window 0, or n_b > kv_len[b]) is zero; unlike rb_attention there is no score
  * clamp, and nothing that stands in a masked position reaches a row. softcap as
  * rb_attention; scale must be positive. max_q bounds the new tokens of any
- * sequence; max_kv is the longest kv_len expected (0: the table's width): it
- * only guides how the work is divided. out must not be an input. */
+ * sequence (0: every sequence that has some is skipped and reported); max_kv is
+ * the longest kv_len expected (0: the table's width): it only guides how the work
+ * is divided. out must not be an input. */
 typedef struct rb_attention_paged_args {
   const void* q;
   void* out;

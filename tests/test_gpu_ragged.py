@@ -741,3 +741,17 @@ def test_append_takes_a_sequence_whole_or_not_at_all(rb, n, kv, positions):
         assert torch.equal(cache.contiguous().view(torch.int16), was.contiguous().view(torch.int16))
     assert torch.equal(q_out[n:], b.q[n:])
     assert torch.equal(q_out[:n], b.q[:n]) if fits else (q_out[:n] == 7.0).all()
+
+
+def test_no_new_tokens_allowed_is_reported(rb):
+    """max_q = 0: every sequence that has a new token is skipped and reported;
+    none has, nothing is."""
+    b = Batch([2, 3], [40, 50], 4, 2, 128, 16, torch.float16)
+    out = b.attend(rb, max_q=0)
+    with pytest.raises(rb.OpFailure, match="bad-shape"):
+        rb.check_device_errors()
+    assert (out == 7.0).all()
+    b.cu.zero_()
+    out = b.attend(rb, max_q=0)
+    rb.check_device_errors()
+    assert (out == 7.0).all()
