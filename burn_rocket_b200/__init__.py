@@ -485,7 +485,8 @@ def attention_paged(q, k_cache, v_cache, page_table, cu_q, kv_len, n_head: int, 
     new tokens were appended. max_q bounds the new tokens of any sequence; max_kv
     is the longest context expected (0: the table's width), which only guides how
     the work is divided. window >= 0 lets a query see its last `window`
-    positions; a query that sees none is zero."""
+    positions (pages behind the window of all new tokens need no page id); a query
+    that sees none is zero."""
     import torch
     op = "attention_paged"
     dev, tokens = _device_of(op, q), q.shape[0]

@@ -427,9 +427,12 @@ tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
       const int page0 = kv.table ? it.ja * per_tile : 0;
       const int pages = kv.table ? (it.kv + page - 1) >> kv.page_shift : 0;
       const int32_t* table = kv.table + it.b * kv.ld_table;
+      int first_key, none;  // that any row of the unit sees
+      visible(it.kv - it.n + it.i0, it.kv, p.a.dlo, p.a.dhi, first_key, none);
       auto fetch = [&](int at) {
         const int idx = page0 + at + lane;
         if (!kv.table || idx >= pages || idx >= (it.jb + 1) * per_tile) return 0;
+        if (idx < first_key >> kv.page_shift) return kv.num_pages;  // behind the window: it may be gone
         const int id = __ldg(table + idx);
         if (static_cast<unsigned>(id) < static_cast<unsigned>(kv.num_pages)) return id;
         atomicOr(err, kErrBadShape);

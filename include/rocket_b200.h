@@ -251,7 +251,9 @@ RB_API int rb_attention_batched(const void* q, int64_t ldq, const void* k, int64
  * slots, pages page_stride elements apart (page_size 16, 32, 64 or 128; head_dim
  * 64 or 128); position j of sequence b lies in slot j % page_size of page
  * page_table[b*ld_table + j/page_size]. Table entries past a sequence's last
- * page are not read, slots past its last position may hold anything.
+ * page are not read, nor, by rb_attention_paged, those of pages that lie behind
+ * the window of all its new tokens (the pages may have been given back); slots
+ * past its last position may hold anything.
  *
  * What the device data says is checked on the device, and what does not fit is
  * reported by rb_check_device_errors (bad-shape): a sequence with bounds outside

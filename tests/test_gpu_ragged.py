@@ -755,3 +755,23 @@ def test_no_new_tokens_allowed_is_reported(rb):
     out = b.attend(rb, max_q=0)
     rb.check_device_errors()
     assert (out == 7.0).all()
+
+
+@pytest.mark.parametrize("q,kv,h,hkv,page,window", [
+    ([1, 1], [700, 90], 16, 8, 16, 100), ([3, 2], [700, 1111], 4, 2, 32, 64), ([40, 33], [700, 95], 16, 8, 16, 100),
+    ([300, 17], [1500, 400], 8, 1, 16, 90), ([200, 150], [3000, 2000], 4, 2, 64, 30), ([20], [9000], 8, 1, 16, 1000)])
+def test_pages_behind_the_window_may_be_gone(rb, q, kv, h, hkv, page, window):
+    """Pages of which no new token sees a key need no page id."""
+    b = Batch(q, kv, h, hkv, 128, page, torch.float16, seed=q[0])
+    for s, (n, m) in enumerate(zip(q, kv)):
+        b.table[s, :max(0, m - n - window + 1) // page] = -1
+    out = b.attend(rb, window=window)
+    rb.check_device_errors()
+    b.verify(out, window=window)
+
+
+SPLIT_MASKED = [
+    # new tokens, keys (few units of many key tiles: cut over a cluster), heads, kv heads, head_dim, masked position
+    (150, 3000, 4, 2, 128, 2990), (150, 3000, 4, 2, 128, 2860), (150, 3000, 4, 2, 64, 2999), (40, 6000, 8, 1, 128, 5990),
+    (600, 1400, 2, 1, 64, 1100),
+]
