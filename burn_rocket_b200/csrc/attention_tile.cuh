@@ -685,7 +685,7 @@ tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUt
         bool need = false;
         if (j == lo) {
           m_used = mt;
-        } else if (!(mt <= m_used + kRescale)) {
+        } else if (valid && !(mt <= m_used + kRescale)) {  // (a row without a query may hold anything, NaN too)
           alpha = ex2(m_used - mt);
           m_used = mt;
           need = true;
