@@ -53,13 +53,14 @@ int check_rows(const char* op, const char* what, const void* p, int64_t ld, int 
   return RB_OK;
 }
 
+// (`empty`: a call without tokens or sequences, whose table may have no address.)
 int check_cache(const char* op, const Heads& h, const void* k, const void* v, int64_t page_stride, int64_t num_pages,
-                int page_size, const int32_t* table, int64_t ld_table, KeyValues* kv) {
+                int page_size, const int32_t* table, int64_t ld_table, bool empty, KeyValues* kv) {
   if (h.d != 64 && h.d != 128)
     return refuse(RB_E_UNSUPPORTED, "%s: head_dim %d (supported: 64, 128)", op, h.d);
   if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128)
     return refuse(RB_E_UNSUPPORTED, "%s: page_size %d (supported: 16, 32, 64, 128)", op, page_size);
-  if (num_pages <= 0 || num_pages > kMaxRows || ld_table <= 0 || !table)
+  if (num_pages <= 0 || num_pages > kMaxRows || (!empty && (ld_table <= 0 || !table)))
     return refuse(RB_E_SHAPE, "%s: num_pages=%lld, page table width %lld", op, (long long)num_pages,
                   (long long)ld_table);
   const int64_t row = static_cast<int64_t>(h.n_kv_heads) * h.d;
@@ -109,7 +110,7 @@ extern "C" int rb_kv_append(const rb_kv_append_args* args, void* stream) {
   KvAppend a{};
   if ((rc = check_common(op, dtype, tokens, batch, h)) != RB_OK ||
       (rc = check_cache(op, h, k_cache, v_cache, page_stride, num_pages, page_size, page_table, ld_table,
-                        &a.cache)) != RB_OK)
+                        tokens == 0 || batch == 0, &a.cache)) != RB_OK)
     return rc;
   if (!(eps >= 0.0f)) return refuse(RB_E_SHAPE, "%s: eps %g", op, static_cast<double>(eps));
   if (tokens == 0 || batch == 0) return RB_OK;
@@ -162,8 +163,8 @@ extern "C" int rb_attention_paged(const rb_attention_paged_args* args, void* str
   const Heads h{n_head, n_kv_heads, head_dim};
   AttnRagged a{};
   if ((rc = check_common(op, dtype, tokens, batch, h)) != RB_OK ||
-      (rc = check_cache(op, h, k_cache, v_cache, page_stride, num_pages, page_size, page_table, ld_table, &a.kv)) !=
-          RB_OK ||
+      (rc = check_cache(op, h, k_cache, v_cache, page_stride, num_pages, page_size, page_table, ld_table,
+                        tokens == 0 || batch == 0, &a.kv)) != RB_OK ||
       (rc = check_softmax(op, scale, softcap)) != RB_OK)
     return rc;
   if (max_q < 0 || max_kv < 0) return refuse(RB_E_SHAPE, "%s: max_q=%lld max_kv=%lld", op, (long long)max_q, (long long)max_kv);

@@ -803,3 +803,19 @@ def test_rows_without_a_query_take_no_part(rb, h, hkv):
     rb.check_device_errors()
     verify_packed(out, lens, q, k, v, h, hkv, d, True, -1, 0.0, torch.float16)
     assert best["nan"] <= 1.07 * best["0.0"], best
+
+
+def test_empty_batches_have_no_table(rb):
+    """No sequence, or none with keys: empty page tables have no address."""
+    cache = torch.zeros(2, 16, 2, 64, device="cuda", dtype=torch.float16)
+    i32 = dict(device="cuda", dtype=torch.int32)
+    ang = torch.zeros(8, 32, device="cuda")
+    for batch in (0, 3):
+        for rows in (0, 5) if batch == 0 else (0,):
+            q, k = (torch.full((rows, n), 3.0, device="cuda", dtype=torch.float16) for n in (256, 128))
+            table, cu, kv = torch.zeros(batch, 0 if batch else 4, **i32), torch.zeros(batch + 1, **i32), torch.zeros(batch, **i32)
+            out = torch.full_like(q, 7.0)
+            assert rb.kv_append(q, k, k, cache, cache.clone(), table, cu, kv, 4, 2, 64, ang, ang, q_out=out) is out
+            assert rb.attention_paged(q, cache, cache, table, cu, kv, 4, 2, 64, 0.1, max_q=1, out=out) is out
+            assert (out == 7.0).all()
+    rb.check_device_errors()

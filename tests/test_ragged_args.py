@@ -124,3 +124,11 @@ def test_python_refusals():
         rb.kv_append(q, q, q, q, q, cu, cu, cu, 2, 2, 128, q, q)
     with pytest.raises(rb.OpFailure, match="CUDA"):
         rb.attention_paged(q, q, q, cu, cu, cu, 2, 2, 128, 0.1, max_q=4)
+
+
+@pytest.mark.parametrize("name,base", [("rb_kv_append", APPEND), ("rb_attention_paged", PAGED)])
+@pytest.mark.parametrize("empty", [dict(batch=0), dict(tokens=0)])
+def test_empty_batches_need_no_table(name, base, empty):
+    """An empty tensor has no address: that of an empty batch is not asked for."""
+    assert call(name, base, table=None, **empty) == _lib.RB_OK
+    assert call(name, base, table=None, ld_table=0, **empty) == _lib.RB_OK
