@@ -119,6 +119,8 @@ extern "C" int rb_kv_append(const rb_kv_append_args* args, void* stream) {
       (rc = check_rows(op, "v", v, ldv, n_kv_heads, head_dim)) != RB_OK ||
       (rc = check_rows(op, "q_out", q_out, ldq_out, n_head, head_dim)) != RB_OK)
     return rc;
+  if (q_out == k || q_out == v || q_out == k_cache || q_out == v_cache)
+    return refuse(RB_E_SHAPE, "%s: q_out may be q, but no other input", op);
   if (q_out == q && ldq_out != ldq) return refuse(RB_E_SHAPE, "%s: q in place needs one row stride", op);
   if (!cu_q || !kv_len || !cos_t || !sin_t || max_pos <= 0 || max_pos > kMaxRows)
     return refuse(RB_E_SHAPE, "%s: null cu_q, kv_len, cos or sin, or max_pos=%lld", op, (long long)max_pos);

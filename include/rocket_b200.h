@@ -276,8 +276,8 @@ RB_API int rb_attention_batched(const void* q, int64_t ldq, const void* k, int64
  * likewise into the cache, its v heads unchanged. The norm is the per-head
  * RMSNorm of rb_qk_norm_rope with weights f32 [head_dim], NULL = none; cos/sin
  * are f32 [max_pos, head_dim/2] as for rb_rope. Arithmetic in f32, one rounding.
- * q_out may be q itself (with ldq_out == ldq). Two tokens must not map to one
- * slot. */
+ * q_out may be q itself (with ldq_out == ldq) but no other input. Two tokens must
+ * not map to one slot. */
 typedef struct rb_kv_append_args {
   const void *q, *k, *v;
   int64_t ldq, ldk, ldv; /* row strides in elements */

@@ -132,3 +132,12 @@ def test_empty_batches_need_no_table(name, base, empty):
     """An empty tensor has no address: that of an empty batch is not asked for."""
     assert call(name, base, table=None, **empty) == _lib.RB_OK
     assert call(name, base, table=None, ld_table=0, **empty) == _lib.RB_OK
+
+
+@pytest.mark.parametrize("where", ["k", "v", "k_cache", "v_cache"])
+def test_rotated_queries_over_another_input_are_refused(where):
+    """q may be rotated in place; over k or v other heads would read what was
+    written, over the cache other tokens' slots would be lost."""
+    base = dict(APPEND, n_kv_heads=16, ldk=2048, ldv=2048, page_stride=16 * 2048, k_cache=P + 512, v_cache=P + 1024)
+    assert call("rb_kv_append", base, q_out=base[where]) == _lib.RB_E_SHAPE
+    assert _lib.last_error().startswith("kv_append: q_out")
