@@ -770,13 +770,6 @@ def test_pages_behind_the_window_may_be_gone(rb, q, kv, h, hkv, page, window):
     b.verify(out, window=window)
 
 
-SPLIT_MASKED = [
-    # new tokens, keys (few units of many key tiles: cut over a cluster), heads, kv heads, head_dim, masked position
-    (150, 3000, 4, 2, 128, 2990), (150, 3000, 4, 2, 128, 2860), (150, 3000, 4, 2, 64, 2999), (40, 6000, 8, 1, 128, 5990),
-    (600, 1400, 2, 1, 64, 1100),
-]
-
-
 @pytest.mark.parametrize("h,hkv", [(12, 4), (14, 2)])
 def test_rows_without_a_query_take_no_part(rb, h, hkv):
     """Groups that do not divide 128 leave rows of a tile without a query: what an
@@ -819,3 +812,141 @@ def test_empty_batches_have_no_table(rb):
             assert rb.attention_paged(q, cache, cache, table, cu, kv, 4, 2, 64, 0.1, max_q=1, out=out) is out
             assert (out == 7.0).all()
     rb.check_device_errors()
+
+
+@pytest.mark.parametrize("q", [[2, 3, 1], [40, 60, 30]])
+def test_rows_of_a_sequence_after_falling_bounds(rb, q):
+    """A sequence whose own bounds are in order is computed though others fall."""
+    b = Batch(q, [140, 150, 160], 4, 2, 128, 16, torch.float16, tail_rows=0)
+    first, n = q[0] + q[1], q[2]
+    b.cu[1] = sum(q)
+    out = b.attend(rb, max_q=max(q))
+    with pytest.raises(rb.OpFailure, match="bad-shape"):
+        rb.check_device_errors()
+    assert (out[:first] == 7.0).all()
+    ref, size = reference(b.q[first:].view(n, 4, 128), b.k[2], b.v[2], band(n, 160, True, -1), 1 / math.sqrt(128), 0)
+    check(out[first:].view(n, 4, 128), ref, size, 160, torch.float16)
+
+
+SPLIT_MASKED = [
+    # new tokens, keys (few units of many key tiles: cut over a cluster), heads, kv heads, head_dim, masked position
+    (150, 3000, 4, 2, 128, 2990), (150, 3000, 4, 2, 128, 2860), (150, 3000, 4, 2, 64, 2999), (40, 6000, 8, 1, 128, 5990),
+    (600, 1400, 2, 1, 64, 1100),
+]
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("n,m,h,hkv,d,at", SPLIT_MASKED)
+def test_masked_values_of_a_cut_unit(rb, n, m, h, hkv, d, at, dtype, value):
+    """A unit cut over a cluster: a key and a value that only later rows see leave
+    the earlier rows alone; windows that pass an early one likewise."""
+    dt = DT[dtype]
+    for window, j in ((-1, at), (m - n // 2, n // 4)):
+        b = Batch([n], [m], h, hkv, d, 32, dt, seed=at)
+        page = b.table[0, j // 32].long()
+        b.v_cache[page, j % 32, 0, 5] = value
+        b.v[0][j, 0, 5] = value
+        out = b.attend(rb, window=window)
+        rb.check_device_errors()
+        seen = band(n, m, True, window)
+        assert seen[:, j].any() and not seen[:, j].all()
+        got = out[:n].view(n, h, d)
+        ref, size = reference(b.q[:n].view(n, h, d), b.k[0], b.v[0], seen, 1 / math.sqrt(d), 0)
+        hit = torch.zeros(n, h, d, dtype=torch.bool, device="cuda")
+        hit[:, :h // hkv, 5] = seen[:, j, None]
+        assert torch.equal(torch.isfinite(got), ~hit)
+        check(got.masked_fill(hit, 0.0), ref.masked_fill(hit, 0.0), size.masked_fill(hit, 0.0), m, dt)
+        # the key too: rows that see it end as their softmax does, the others are untouched
+        b.k_cache[page, j % 32, 0] = value
+        again = b.attend(rb, window=window)[:n].view(n, h, d)
+        rb.check_device_errors()
+        clean = ~seen[:, j]
+        check(again[clean], ref[clean], size[clean], m, dt)
+        assert torch.isnan(again[~clean][:, :h // hkv]).all()  # infinite scores of both signs in a row's sum
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("h,hkv,d,causal", [(4, 2, 72, True), (2, 2, 72, False), (4, 2, 128, True), (2, 1, 64, True)])
+def test_masked_values_of_a_cut_packed_unit(rb, h, hkv, d, causal, dtype):
+    """The same for one packed sequence of 1500 tokens, in the middle and in the
+    last tile; the bidirectional form masks by its window."""
+    dt, n, window = DT[dtype], 1500, -1 if causal else 300
+    for j in (700, 1490):
+        cu, q, k, v = packed_state([n], h, hkv, d, dt, j)
+        v[j, 3] = math.nan
+        k[j] = math.inf
+        out = torch.full((q.shape[0], h * d), 7.0, device="cuda", dtype=dt)
+        rb.attention_packed(q, k, v, cu, h, hkv, d, 1 / math.sqrt(d), is_causal=causal, window=window, out=out)
+        rb.check_device_errors()
+        seen = band(n, n, causal, window)
+        clean = ~seen[:, j]
+        assert clean.any() and not clean.all()
+        vv, kk = v[:n].reshape(n, hkv, d), k[:n].reshape(n, hkv, d).clone()
+        kk[j] = 0.0
+        ref, size = reference(q[:n].reshape(n, h, d), kk, vv, seen, 1 / math.sqrt(d), 0)
+        got = out[:n].view(n, h, d)
+        check(got[clean], ref[clean], size[clean], n, dt)
+        assert torch.isnan(got[~clean]).all()  # an infinite score of either sign among the products of a row
+        assert (out[n:] == 7.0).all()
+
+
+def test_offsets_past_32_bits(rb):
+    """Slots more than 2^31 elements into the cache: appended and attended."""
+    h, hkv, d, page, dt = 8, 8, 128, 128, torch.bfloat16
+    pages = (1 << 31) // (page * hkv * d) + 40
+    k_cache, v_cache = (torch.empty(pages, page, hkv, d, device="cuda", dtype=dt) for _ in range(2))
+    total = [400, 300]
+    used = torch.arange(pages - 10, pages, device="cuda", dtype=torch.int32)
+    table = torch.stack([used[:4], used[4:8]]).contiguous()
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(sum(total), 3 * h * d, generator=g, device="cuda").to(dt)
+    q, k, v = x.split([h * d] * 3, dim=1)
+    cu = torch.tensor([0, 400, 700], device="cuda", dtype=torch.int32)
+    kv_len = torch.tensor(total, device="cuda", dtype=torch.int32)
+    cos, sin = torch.ones(400, d // 2, device="cuda"), torch.zeros(400, d // 2, device="cuda")
+    qr = rb.kv_append(q, k, v, k_cache, v_cache, table, cu, kv_len, h, hkv, d, cos, sin)
+    assert torch.equal(qr, q)
+    out = rb.attention_paged(qr, k_cache, v_cache, table, cu, kv_len, h, hkv, d, 1 / math.sqrt(d), max_q=400)
+    last = torch.tensor([399, 699], device="cuda")
+    one = rb.attention_paged(q[last].contiguous(), k_cache, v_cache, table, torch.arange(3, device="cuda", dtype=torch.int32),
+                             kv_len, h, hkv, d, 1 / math.sqrt(d), max_q=1)
+    rb.check_device_errors()
+    for b, r in enumerate((slice(0, 400), slice(400, 700))):
+        n = total[b]
+        assert torch.equal(k_cache[table[b].long()].reshape(-1, hkv * d)[:n], k[r])
+        ref, size = reference(q[r].reshape(n, h, d), k[r].reshape(n, hkv, d), v[r].reshape(n, hkv, d), band(n, n, True, -1),
+                              1 / math.sqrt(d), 0)
+        check(out[r].view(n, h, d), ref, size, n, dt)
+        check(one[b].view(1, h, d), ref[-1:], size[-1:], n, dt)
+
+
+def test_packed_prompts_of_a_rotary_model(rb):
+    """Prompts without a cache: one qk_norm_rope over the packed rows with the
+    angle rows gathered by position, then attention_packed; equal to the cache's
+    way (kv_append)."""
+    from burn_rocket_b200 import _lib
+    from burn_rocket_b200.qwen3 import rope_tables
+    lens, h, hkv, d, dt = [70, 1, 0, 133], 16, 8, 128, torch.float16
+    n = sum(lens)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    qkv = torch.randn(n, (h + 2 * hkv) * d, generator=g, device="cuda").to(dt)
+    wq, wk = (1 + 0.1 * torch.randn(d, generator=g, device="cuda") for _ in range(2))
+    cos, sin = (torch.from_numpy(x).cuda() for x in rope_tables(256, d, 1e6))
+    cu = torch.tensor([0] + lens, device="cuda").cumsum(0).to(torch.int32)
+    pos = torch.cat([torch.arange(m, device="cuda") for m in lens])
+    cos_rows, sin_rows = cos[pos].contiguous(), sin[pos].contiguous()
+    table = torch.arange(40, device="cuda", dtype=torch.int32).view(4, 10)
+    k_cache, v_cache = (torch.zeros(40, 16, hkv, d, device="cuda", dtype=dt) for _ in range(2))
+    q, k, v = qkv.split([h * d, hkv * d, hkv * d], dim=1)
+    kv_len = torch.tensor(lens, device="cuda", dtype=torch.int32)
+    qr = rb.kv_append(q, k, v, k_cache, v_cache, table, cu, kv_len, h, hkv, d, cos, sin, wq, wk)
+    kr = torch.cat([k_cache[table[b].long()].reshape(-1, hkv * d)[:m] for b, m in enumerate(lens)])
+    rb._check(_lib.load().rb_qk_norm_rope(qkv.data_ptr(), qkv.shape[1], n, h, hkv, d, wq.data_ptr(), wk.data_ptr(), 1e-6,
+                                          cos_rows.data_ptr(), sin_rows.data_ptr(), n, rb._stream_ptr(None)), "qk_norm_rope")
+    # two f32 evaluations of one value round to neighbours at most
+    for x, ref in ((qr, q), (kr, k)):
+        assert ((x.float() - ref.float()).abs() <= 2.0 ** -10 * ref.float().abs() + 2.0 ** -19).all()
+    out = rb.attention_packed(q, k, v, cu, h, hkv, d, 1 / math.sqrt(d))
+    rb.check_device_errors()
+    verify_packed(out, lens, q, k, v, h, hkv, d, True, -1, 0.0, dt)
