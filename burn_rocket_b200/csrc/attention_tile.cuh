@@ -56,8 +56,6 @@ constexpr int kSoftWarp0 = 4;
 constexpr int kSoftThreads = 8 * 32;
 constexpr int kLaunchRegs = 168, kRoleRegs = 104, kSoftRegs = 200;
 static_assert(kRoleRegs + 2 * kSoftRegs <= 3 * kLaunchRegs, "the shares come from the launch's registers");
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kRescale = 8.0f;  // log2 units
 
 struct TileParams {
   AttnRagged a;
@@ -101,11 +99,6 @@ struct Item {
   int lo[2], hi[2];  // a slot's key tiles (empty when lo > hi)
 };
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // NaN if any operand is: a NaN score has to show in its row.
 __device__ __forceinline__ float max2n(float a, float b) {
   float d;
@@ -118,26 +111,6 @@ __device__ __forceinline__ float max3n(float a, float b, float c) {
   return d;
 }
 
-template <bool BF16>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  if (BF16) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-__device__ __forceinline__ uint32_t cluster_size() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ float ld_cluster(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
-}
 __device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"

@@ -76,6 +76,11 @@ __device__ __forceinline__ void visible(int pos, int kv, int dlo, int dhi, int& 
   hi = dhi >= kRaggedNoBound ? kv - 1 : min(kv - 1, pos + dhi);
 }
 
+constexpr float kLog2e = 1.4426950408889634f;
+// How far (in log2) a running maximum may rise above the exponent base before
+// the base follows: weights stay below 2^8, within f16, and few steps rescale.
+constexpr float kRescale = 8.0f;
+
 template <bool BF16>
 __device__ __forceinline__ float h2f(uint16_t x) {
   if (BF16) return __uint_as_float(static_cast<uint32_t>(x) << 16);
@@ -85,6 +90,32 @@ template <bool BF16>
 __device__ __forceinline__ uint16_t f2h(float x) {
   if (BF16) return __bfloat16_as_ushort(__float2bfloat16_rn(x));
   return __half_as_ushort(__float2half_rn(x));
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if (BF16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
 }
 
 // One query row by one warp, from the definition: scores, softmax statistics
