@@ -513,7 +513,9 @@ def attention_packed(q, k, v, cu_seqlens, n_head: int, n_kv_heads: int, head_dim
     prompts of different lengths, rb_attention_packed): rows cu_seqlens[b] ..
     cu_seqlens[b+1] (int32 [batch+1]) of q [tokens, n_head*head_dim] and of k, v
     [tokens, n_kv_heads*head_dim] belong to sequence b. window >= 0: the last
-    `window` keys (causal), or |t - j| <= window."""
+    `window` keys (causal), or |t - j| <= window. For a rotary model q and k come
+    rotated: rb_qk_norm_rope with seq = tokens and the angle rows gathered by
+    position does so for packed rows."""
     import torch
     op = "attention_packed"
     dev, tokens = _device_of(op, q), q.shape[0]

@@ -10,9 +10,10 @@
 //     go to its ring of shared-memory stages by cp.async, 16 bytes a lane,
 //     zero-filled where a key is out of every row's sight, so nothing that lies in
 //     unused slots is ever read.
-//   * S = Q K^T and O += P V by m16n8k16 with f32 accumulation; the online
-//     softmax keeps running row maxima and sums in f32, the exponent base moving
-//     only when a maximum exceeds it by 2^8.
+//   * S = Q K^T and O += P V by m16n8k16 with f32 accumulation, P rounded to the
+//     16-bit type (pack2 says why); the online softmax keeps running row maxima
+//     and sums in f32, the exponent base moving only when a maximum exceeds it by
+//     2^8.
 //   * The blocks of a (sequence, KV head) go round-robin to the warps of a
 //     cluster of 1 to 16 CTAs, whose partial (O, m, l) are merged through
 //     distributed shared memory: no global workspace, no second kernel, nothing
@@ -356,6 +357,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2) decode_kernel(const __grid_con
 // 41, 37, 43 us; 64 x 4096: 184, 197, 209, 238; 3 x 33000 sizes 8, 10, 12, 16:
 // 84, 80, 92, 96 (sizes above 10 leave fewer than 24 clusters resident); 64
 // sequences of 33 to 8100 keys x 4 heads 1, 2, 3, 4, 8: 147, 109, 119, 125, 158.
+// The constants below are fitted to these; between them the chosen sizes were
+// timed, not the others: 8, 16, 32 and 48 sequences of 300 to 8000 keys x 8 heads
+// take 2.2, 1.3, 1.1 and 1.1 times the bytes at the copy rate, 128 and 256 of 33
+// to 4000 x 4 heads 1.1.
 static int pick_ranks(const int* active, int64_t units, int batch, double keys, int d) {
   const double key_ns = 14.0 * d / 128;
   const double all_ns = 0.6 * units * keys * d * 4 / 6300.0 * active[1];  // (lengths vary: most lie below the longest)

@@ -92,6 +92,12 @@ __device__ __forceinline__ uint16_t f2h(float x) {
   return __half_as_ushort(__float2half_rn(x));
 }
 
+// Two softmax weights (or outputs) as 16-bit values. A weight is rounded before
+// P.V because the products take operands of V's type (TF32 would hold no more bits
+// than f16, at half the rate and with V widened); its half step, 2^-11 in f16 and
+// 2^-8 in bf16, enters the output as a mean over the keys. The weights' sum is
+// taken before the rounding, in f32. Against 64 bits an output is off by up to 1.4
+// times what a form in 32 bits with one rounding at the end is.
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   if (BF16) {
